@@ -53,6 +53,7 @@ constexpr int kAttnMaxStages = 6;
 constexpr int kTileKeys = 128;
 constexpr int kStageBytes = 2 * kTileKeys * 128;  // K tile + V tile
 constexpr int kMaxTilesPerCta = 160;
+constexpr int kPageIds = 2 * kMaxTilesPerCta;  // page ids a CTA keeps in shared memory: every tile's with pages of 64 and more
 constexpr float kNeg = -1.0e30f;
 constexpr float kPScale = 256.0f;  // p in [0, 1] is stored as p * 256 (E4M3 / E5M2 range)
 
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[4 * kAttnMaxStages + 2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int page_ids[kMaxTilesPerCta * 2];
+    __shared__ int page_ids[kPageIds];
     __shared__ __align__(16) float wred_s[PBUF][4][NR];  // per-warp maxima of a tile (alternating buffers)
     auto& wred = wred_s[0];
     __shared__ float m_s[NR], alpha_s[PBUF][NR], mrg_m[NR], mrg_l[NR];
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int pg = t_begin * ppt + k;
-                    int id = (k < ppt && pg < p.max_pages) ? p.page_table[b * p.max_pages + pg] : -1;
+                    int id = (k < ppt && pg < p.max_pages) ? p.page_table[static_cast<size_t>(b) * p.max_pages + pg] : -1;
                     if (id >= p.num_pages || id < -1) id = -1;  // reported by the table fill below
                     ids[k] = id;
                 }
@@ -268,15 +269,17 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
             }
         }
     }
-    for (int i = tid; i < nt * ppt && tid < NTHR_F; i += NTHR_F) {
+    auto page_of = [&](int i) {  // physical page i of this CTA's tiles (tile i / ppt), -1 = none: its keys read as zeros
         const int pg = t_begin * ppt + i;
-        int id = pg < p.max_pages ? p.page_table[b * p.max_pages + pg] : -1;
+        int id = pg < p.max_pages ? p.page_table[static_cast<size_t>(b) * p.max_pages + pg] : -1;
         if (id >= p.num_pages || id < -1) {
             report(p.status, MSK_ERR_BOUNDS, where | 2, id, p.num_pages);
             id = -1;
         }
-        page_ids[i] = id;
-    }
+        return id;
+    };
+    const int n_ids = min(nt * ppt, kPageIds);
+    for (int i = tid; i < n_ids && tid < NTHR_F; i += NTHR_F) page_ids[i] = page_of(i);
     for (int i = tid; i < (1 + PBUF) * QP_BYTES / 16 && tid < NTHR_F; i += NTHR_F)
         reinterpret_cast<uint4*>(g_q)[i] = make_uint4(0, 0, 0, 0);
     if (tid < NR) m_s[tid] = kNeg;
@@ -298,7 +301,10 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
         const uint32_t bar = values ? full_v(s) : full(s);
         mbar_expect_tx(bar, kTileKeys * 128);
         for (int j = 0; j < ppt; ++j)
-            tma_load_4d(dst + j * p.page_size * 128, values ? &tm_v : &tm_k, bar, 0, h, 0, page_ids[i * ppt + j]);
+            // (small pages over a long context: ids beyond the shared table come from the page table itself; the copying
+            // thread runs two tiles ahead, which hides the read)
+            tma_load_4d(dst + j * p.page_size * 128, values ? &tm_v : &tm_k, bar, 0, h, 0,
+                        i * ppt + j < kPageIds ? page_ids[i * ppt + j] : page_of(i * ppt + j));
     };
     // `slot`: ring slot of tile i (i % nst; the roles count it instead of dividing)
     auto issue_mma1 = [&](int i, int slot, uint32_t done) {  // S^T = K . q^T into score buffer i & 1

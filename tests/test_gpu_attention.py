@@ -101,6 +101,14 @@ def test_attention_page_sizes(page):
     _check(data, out, k_new, v_new, f"page {page}")
 
 
+@pytest.mark.parametrize("page,q_len", [(8, 1), (16, 1), (16, 8), (32, 1)])
+def test_attention_small_pages_over_a_long_context(page, q_len):
+    """More pages per CTA than the 320 ids it keeps in shared memory (one chunk: 5200 keys are 650, 325 and 163 pages)."""
+    data = oattn.make_input(2, [5200, 5130], seed=page + q_len, q_len=q_len, hq=8, hkv=1, page=page, window=0, rope_theta=0.0)
+    out, k_new, v_new, _ = _run(data, chunks=1)
+    _check(data, out, k_new, v_new, f"page {page}, long")
+
+
 def test_attention_reference_golden(golden):
     """The reference's own outputs (head_dim 128 cases of tests/golden/attention.pt)."""
     n = 0
