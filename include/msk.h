@@ -87,7 +87,7 @@ int msk_proj_scratch_bytes(int M, int N, int K, int splits, int token_splits, si
  * attention over a paged FP8-E4M3 KV cache: per-head RMSNorm of q and k, q * qk_scale_factor,
  * interleaved RoPE, the new tokens' K/V quantised and written into the cache at `cache_loc`,
  * softmax(q.k * sm_scale) over the visible keys (sliding window: a token and the window-1 before it;
- * window 0 = all), output RMSNorm per head times sigmoid(gate), BF16.
+ * window 0 = all; with a window, the first `sinks` positions as well), output RMSNorm per head times sigmoid(gate), BF16.
  * Stands in for muse_attention_decode/submission.py `kernel_fn` (:2363-2372) and the kernels behind it
  * (`attnc_kernel` :1604-1856, `attnpcc_kernel` :1915-2284, `attn_kernel` + `_prep` + `_attn_combine`
  * :293-539,115-173); the fields mirror its `Inputs` / `Config` (:37-65).
@@ -114,6 +114,8 @@ typedef struct {
     int issuers;              /* MMA-issuing warps beside the arithmetic warps: 1; 0 = pick */
     int pdl;
     int row_groups;           /* sets of four arithmetic warps that split the 8 L query rows of a KV head: 2 (decode), 4 (verify); 0 = pick */
+    int sinks;                /* with a window: positions [0, sinks) stay visible to every token (0 = none); pages that lie
+                                 wholly between the sinks and the window are not read, their table entries may be -1 */
 } MskAttnParams;
 
 int msk_attn_decode(const MskAttnParams* p, int* status, void* stream);
@@ -274,6 +276,7 @@ typedef struct {
     int attn_chunks, attn_stages, attn_issuers, qkv_splits, o_splits;
     int attn_row_groups;
     int pdl;                       /* also chain the first kernel to whatever precedes it */
+    int sinks;                     /* as in MskAttnParams */
 } MskLayerFront;
 
 int msk_layer_front(const MskLayerFront* p, int* status, void* stream);

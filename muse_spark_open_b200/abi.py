@@ -144,6 +144,7 @@ class AttnParams(C.Structure):
         ("num_pages", C.c_int), ("window", C.c_int),
         ("qk_scale_factor", C.c_float), ("sm_scale", C.c_float),
         ("chunks", C.c_int), ("stages", C.c_int), ("issuers", C.c_int), ("pdl", C.c_int), ("row_groups", C.c_int),
+        ("sinks", C.c_int),
     ]
 
 
@@ -186,7 +187,7 @@ class LayerFront(C.Structure):
         ("logits", C.c_void_p), ("top_k", C.c_int), ("topk_ids", C.c_void_p), ("topk_weights", C.c_void_p),
         ("attn_chunks", C.c_int), ("attn_stages", C.c_int), ("attn_issuers", C.c_int), ("qkv_splits", C.c_int),
         ("o_splits", C.c_int), ("attn_row_groups", C.c_int),
-        ("pdl", C.c_int),
+        ("pdl", C.c_int), ("sinks", C.c_int),
     ]
 
 

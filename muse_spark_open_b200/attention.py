@@ -3,6 +3,7 @@
 `kernel_fn(data) -> bf16 [B, L, Hq*d]` with the `Inputs` / `Config` fields of
 muse_attention_decode/submission.py:37-65; the new tokens' K/V are written into
 `data["k_cache"]` / `data["v_cache"]` in place at `data["cache_loc"]`, like the reference.
+With a window, `config["sinks"]` (default 0) first positions stay visible to every token.
 Nothing derived from `data` is cached between calls; only the RoPE frequency table (a function of
 theta and head_dim) is kept per device.
 """
@@ -42,6 +43,7 @@ def launch(qkv2d: torch.Tensor, out2d: torch.Tensor, data: dict, cfg: dict, chun
     p.inv_freq = abi.ptr(f) if f is not None else None
     p.B, p.L, p.Hq, p.Hkv, p.d = cfg["batch"], cfg["q_len"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"]
     p.page_size, p.num_pages, p.window = cfg["page_size"], kc.shape[0], cfg["window"]
+    p.sinks = cfg.get("sinks", 0)
     p.qk_scale_factor, p.sm_scale = cfg["qk_scale_factor"], cfg["sm_scale"]
     p.chunks, p.stages, p.issuers, p.pdl, p.row_groups = chunks, stages, issuers, int(pdl), row_groups
     st = abi.status_for(qkv2d.device)

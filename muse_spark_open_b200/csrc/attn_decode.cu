@@ -40,6 +40,9 @@
 // Merge: every CTA pushes its (m, l, o) partials for the query rows another CTA owns into that
 // CTA's shared memory (DSMEM), one cluster barrier, then each owner merges, applies the per-head
 // RMSNorm and the sigmoid gate and stores BF16.
+// With a window, the first `sinks` positions stay visible to every token: a key at position s is seen by the token at
+// position t when s <= t and (s > t - window or s < sinks).  Only the tiles that hold such keys are read (the pages in
+// between may be gone: table entry -1), so a long context costs window + sinks keys.
 // Roofline: HBM (K and V bytes of the visible keys, read once).
 #include <cuda_fp8.h>
 
@@ -71,7 +74,7 @@ struct AttnArgs {
     int max_pages;
     const long long* cache_loc;
     const float* inv_freq;
-    int B, Hq, Hkv, page_size, num_pages, window, nstages, longest_first;
+    int B, Hq, Hkv, page_size, num_pages, window, sinks, nstages, longest_first;
     float qk_scale_factor, sm_scale, q_split_scale;
     int* status;
 };
@@ -224,18 +227,25 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     }
     const int seq = p.seq_lens[b];
     const int W = p.window;
+    // The tiles with visible keys: those of the first `sinks` positions that lie wholly before the window's first tile,
+    // then the window's.  The chunks of the cluster split this list; `gap` tiles between the two parts are skipped.
+    const int snk = W > 0 ? p.sinks : 0;
     const int lo_all = W > 0 ? max(0, seq - W + 1) : 0;
-    const int tiles_total = seq > 0 ? ((seq - 1) / kTileKeys - lo_all / kTileKeys + 1) : 0;
     const int t_first = lo_all / kTileKeys;
+    const int sink_tiles = min((min(snk, seq) + kTileKeys - 1) / kTileKeys, t_first);
+    const int gap = t_first - sink_tiles;
+    const int tiles_total = seq > 0 ? ((seq - 1) / kTileKeys - t_first + 1 + sink_tiles) : 0;
     const int per = (tiles_total + C - 1) / C;
-    const int t_begin = t_first + rank * per;
-    int nt = min(per, t_first + tiles_total - t_begin);
+    const int v_begin = rank * per;
+    auto tile_of = [&](int i) { return v_begin + i + (v_begin + i >= sink_tiles ? gap : 0); };  // tile i of this CTA
+    int nt = min(per, tiles_total - v_begin);
     if (nt < 0) nt = 0;
     if (nt > kMaxTilesPerCta) {
         if (tid == 0) report(p.status, MSK_ERR_CAPACITY, where | 1, nt, kMaxTilesPerCta);
         nt = kMaxTilesPerCta;
     }
-    const int ppt = kTileKeys / p.page_size;  // pages per tile
+    const int ppt = kTileKeys / p.page_size;  // pages per tile, a power of two
+    const int ppt_log = 31 - __clz(ppt);
     // The copying warp only arrives at the CTA's first barrier (it made the mbarriers, the others wait for them
     // there) and takes no part in the fills below; its thread fetches the page ids of the first tile itself and
     // starts that copy at once instead of waiting for the shared table.
@@ -251,7 +261,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                 int ids[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const int pg = t_begin * ppt + k;
+                    const int pg = tile_of(0) * ppt + k;
                     int id = (k < ppt && pg < p.max_pages) ? p.page_table[static_cast<size_t>(b) * p.max_pages + pg] : -1;
                     if (id >= p.num_pages || id < -1) id = -1;  // reported by the table fill below
                     ids[k] = id;
@@ -270,7 +280,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
         }
     }
     auto page_of = [&](int i) {  // physical page i of this CTA's tiles (tile i / ppt), -1 = none: its keys read as zeros
-        const int pg = t_begin * ppt + i;
+        const int pg = tile_of(i >> ppt_log) * ppt + (i & (ppt - 1));
         int id = pg < p.max_pages ? p.page_table[static_cast<size_t>(b) * p.max_pages + pg] : -1;
         if (id >= p.num_pages || id < -1) {
             report(p.status, MSK_ERR_BOUNDS, where | 2, id, p.num_pages);
@@ -533,14 +543,15 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
         for (int i = 0; i < nt; ++i) {
             ok = mbar_wait(sdone(slot), ph, p.status, where | 5) && ok;
             tc_fence_after();
-            const int pos = (t_begin + i) * kTileKeys + ktid;  // this thread's key position
+            const int pos = tile_of(i) * kTileKeys + ktid;  // this thread's key position
+            const bool sink = pos < snk;
             float skeep[NRG];
 #pragma unroll
             for (int c0 = 0; c0 < NRG; c0 += BR) {
                 float sc[BR];
                 load_scores(i, r_lo + c0, sc);
                 const int j = (r_lo + c0) >> 3;
-                const bool vis = pos < seq && (W == 0 || pos > seq + j - W);
+                const bool vis = pos < seq && (W == 0 || pos > seq + j - W || sink);
 #pragma unroll
                 for (int g = 0; g < BR; ++g) {
                     const float sv = vis ? sc[g] * s_scale : kNeg;
@@ -578,8 +589,9 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                     m_s[r] = mn;
                 }
             }
-            // V rows past the cached length may hold anything (even NaN bytes): zero them so that 0 * V stays 0
-            if (rg == 0 && pos >= seq) {
+            // V rows that no query row sees -- past the cached length, or between the sinks and the window -- may hold
+            // anything (even NaN bytes): zero them so that 0 * V stays 0
+            if (rg == 0 && (pos >= seq || (W > 0 && pos <= seq - W && !sink))) {
                 ok = mbar_wait(full_v(slot), ph, p.status, where | 12) && ok;
                 uint8_t* vrow = gbase + slot * kStageBytes + kTileKeys * 128 + ktid * 128;
 #pragma unroll
@@ -592,7 +604,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
 #pragma unroll
             for (int g = 0; g < NRG; g += 2) {  // two rows per conversion instruction
                 const int n = r_lo + g;
-                const bool vis = pos < seq && (W == 0 || pos > seq + (n >> 3) - W);  // rows n and n + 1: same token
+                const bool vis = pos < seq && (W == 0 || pos > seq + (n >> 3) - W || sink);  // rows n and n + 1: same token
                 const float m0 = L == 1 ? m_r[g] : m_s[n], m1 = L == 1 ? m_r[g + 1] : m_s[n + 1];
                 const float a0 = L == 1 ? alpha_r[g] : alpha_s[i & 1][n], a1 = L == 1 ? alpha_r[g + 1] : alpha_s[i & 1][n + 1];
                 const float pr0 = vis ? ex2(skeep[g] - m0) : 0.0f;
@@ -682,7 +694,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                 const uint32_t qq = *reinterpret_cast<const uint32_t*>(qf + n * 128 + d);
                 acc += bf16lo(qq) * knew[r * 128 + d] + bf16hi(qq) * knew[r * 128 + d + 1];
             }
-            const bool vis = r <= j && (W == 0 || r > j - W);
+            const bool vis = r <= j && (W == 0 || r > j - W || seq + r < snk);
             sc_tail[n][r] = vis ? acc * t_scale : kNeg;
         }
         csync();
@@ -790,7 +802,8 @@ int launch_attn(const MskAttnParams* q, int* status, cudaStream_t stream) {
     constexpr int kColsHost = attn_tmem_cols(L);
     const int tile_cap = (q->max_pages * q->page_size + kTileKeys - 1) / kTileKeys;
     int tiles_max = tile_cap;
-    if (q->window > 0) tiles_max = min(tiles_max, q->window / kTileKeys + 2);
+    if (q->window > 0)  // the window's tiles and the sinks', each at an unknown offset
+        tiles_max = min(static_cast<long long>(tiles_max), static_cast<long long>(q->window / kTileKeys) + q->sinks / kTileKeys + 2 + (q->sinks > 0 ? 1 : 0));
     if (tiles_max < 1) tiles_max = 1;
     // the ring needs 3 slots: a tile's slot is refilled one iteration after its tile (finish_tile runs late),
     // and the next tile's scores are issued one iteration early
@@ -841,7 +854,7 @@ int launch_attn(const MskAttnParams* q, int* status, cudaStream_t stream) {
     a.max_pages = q->max_pages, a.cache_loc = reinterpret_cast<const long long*>(q->cache_loc), a.inv_freq = q->inv_freq;
     a.B = q->B, a.Hq = q->Hq, a.Hkv = q->Hkv, a.page_size = q->page_size, a.num_pages = q->num_pages;
     a.longest_first = (q->B <= 256 && q->B * q->Hkv * C > resident * 148) ? 1 : 0;
-    a.window = q->window, a.nstages = nst, a.qk_scale_factor = q->qk_scale_factor, a.sm_scale = q->sm_scale;
+    a.window = q->window, a.sinks = q->sinks, a.nstages = nst, a.qk_scale_factor = q->qk_scale_factor, a.sm_scale = q->sm_scale;
     // largest power of two that keeps |q| * scale <= 448 (|q| <= qk_scale_factor * sqrt(128) after RMSNorm)
     float qs = 1.0f;
     const float qmax = fabsf(q->qk_scale_factor) * 11.3137085f;
@@ -889,6 +902,7 @@ extern "C" int msk_attn_decode(const MskAttnParams* q, int* status, void* stream
     if (q->d != 128 || q->Hkv < 1 || q->Hq != 8 * q->Hkv || q->B < 1) return MSK_ERR_UNSUPPORTED;
     if (q->page_size < 8 || q->page_size > 128 || (q->page_size & (q->page_size - 1)) != 0) return MSK_ERR_UNSUPPORTED;
     if (q->issuers != 0 && q->issuers != 1) return MSK_ERR_INVALID;
+    if (q->window < 0 || q->sinks < 0) return MSK_ERR_INVALID;
     if (q->row_groups != 0 && q->row_groups != (q->L == 1 ? 2 : 4)) return MSK_ERR_INVALID;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (q->L == 1) return launch_attn<1, 2>(q, status, s);  // 8 arithmetic warps + MMA warp + copying warp, 2 CTAs per SM

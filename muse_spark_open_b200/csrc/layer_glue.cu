@@ -516,7 +516,7 @@ extern "C" int msk_layer_front(const MskLayerFront* f, int* status, void* stream
     a.k_cache = f->k_cache, a.v_cache = f->v_cache, a.k_scale = f->k_scale, a.v_scale = f->v_scale;
     a.seq_lens = f->seq_lens, a.page_table = f->page_table, a.max_pages = f->max_pages, a.cache_loc = f->cache_loc;
     a.inv_freq = f->inv_freq, a.B = f->B, a.L = f->L, a.Hq = f->Hq, a.Hkv = f->Hkv, a.d = f->d;
-    a.page_size = f->page_size, a.num_pages = f->num_pages, a.window = f->window;
+    a.page_size = f->page_size, a.num_pages = f->num_pages, a.window = f->window, a.sinks = f->sinks;
     a.qk_scale_factor = f->qk_scale_factor, a.sm_scale = f->sm_scale;
     a.chunks = f->attn_chunks, a.stages = f->attn_stages, a.issuers = f->attn_issuers, a.row_groups = f->attn_row_groups, a.pdl = 1;
     rc = msk_attn_decode(&a, status, stream);

@@ -70,6 +70,7 @@ def fill_front(f: abi.LayerFront, data: dict, state: dict, buf: dict, tune: dict
     f.Hq, f.Hkv, f.d = cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"]
     f.page_size, f.num_pages, f.max_pages = cfg["page_size"], data["k_cache"].shape[0], data["page_table"].shape[1]
     f.window, f.qk_scale_factor, f.sm_scale, f.norm_eps = cfg["window"], cfg["qk_scale_factor"], cfg["sm_scale"], RMS_EPS
+    f.sinks = cfg.get("sinks", 0)
     f.stream = abi.ptr(data["stream"])
     f.k_cache, f.v_cache = abi.ptr(data["k_cache"]), abi.ptr(data["v_cache"])
     f.k_scale, f.v_scale = abi.ptr(data["k_scale"]), abi.ptr(data["v_scale"])

@@ -104,10 +104,69 @@ def ref_kernel(data, new_kv=None, scale_after_rope: bool = False):
             p = seq + j
             lo = max(0, p - cfg["window"] + 1) if cfg["window"] else 0
             kb, vb = keys[lo:p + 1], vals[lo:p + 1]
+            if cfg.get("sinks", 0):  # the first positions that stay visible under a window
+                n = min(cfg["sinks"], lo)
+                kb, vb = torch.cat([keys[:n], kb]), torch.cat([vals[:n], vb])
             s = torch.einsum("kgd,tkd->kgt", q[b, j].view(hkv, grp, d), kb) * cfg["sm_scale"]
             out[b, j] = torch.einsum("kgt,tkd->kgd", s.softmax(-1), vb).reshape(hq, d)
     out = rms(out) * torch.sigmoid(gate.float()).view(b_n, l_n, hq, d)
     return out.reshape(b_n, l_n, hq * d), k_new, v_new
+
+
+def ref_stream(data, new_kv=None):
+    """(out fp64 [T, Hq*d], k_new, v_new e4m3 [T, Hkv, d]) for new tokens of any number per request, in 64 bits: request b
+    brings the rows cu_seqlens_q[b] .. cu_seqlens_q[b+1] of qkv behind its seq_lens[b] cached tokens.  A token at position
+    t sees s <= t with window == 0 or s > t - window or s < sinks.  Queries are rounded to BF16, new keys and values to
+    E4M3, like `ref_kernel`; the RoPE angle is the exact product of the position and the FP32 frequency.  With new_kv the
+    tokens attend those entries as their own.  Page-table entries of positions no token sees are not looked at.
+    """
+    cfg = data["config"]
+    hq, hkv, d, w, sinks = cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"], cfg["window"], cfg.get("sinks", 0)
+    size, grp = cfg["page_size"], hq // hkv
+    cu = data["cu_seqlens_q"].tolist()
+    x = data["qkv"].reshape(-1, (2 * hq + 2 * hkv) * d)[:cu[-1]].double()
+    seq = data["seq_lens"].long()
+    pos = torch.cat([torch.arange(int(seq[b]), int(seq[b]) + cu[b + 1] - cu[b]) for b in range(len(cu) - 1)])
+
+    def norm_rope(u, scale):
+        u = u / torch.sqrt(u.pow(2).mean(-1, keepdim=True) + RMS_EPS) * scale
+        if cfg["rope_theta"]:
+            freq = (1.0 / (cfg["rope_theta"] ** (torch.arange(0, d, 2).float() / d))).double()
+            ang = (pos.double()[:, None] * freq)[:, None, :]
+            a, b = u[..., 0::2], u[..., 1::2]
+            u = torch.stack((a * ang.cos() - b * ang.sin(), a * ang.sin() + b * ang.cos()), -1).flatten(-2)
+        return u
+
+    t = x.shape[0]
+    q = norm_rope(x[:, :hq * d].view(t, hq, d), cfg["qk_scale_factor"]).to(torch.bfloat16).double()
+    ks, vs = data["k_scale"].double(), data["v_scale"].double()
+    k_new = (norm_rope(x[:, hq * d:(hq + hkv) * d].view(t, hkv, d), 1.0) / ks).clamp(-448, 448).to(FP8)
+    v_new = (x[:, (hq + hkv) * d:(hq + 2 * hkv) * d].view(t, hkv, d) / vs).clamp(-448, 448).to(FP8)
+    if new_kv is not None:
+        k_new, v_new = (u.reshape(t, hkv, d) for u in new_kv)
+    kc, vc = data["k_cache"].view(-1, hkv, d), data["v_cache"].view(-1, hkv, d)
+    out = torch.empty((t, hq, d), dtype=torch.float64)
+    for b in range(len(cu) - 1):
+        c, n = int(seq[b]), cu[b + 1] - cu[b]
+        if n == 0:
+            continue
+        past = torch.arange(c)
+        if w:
+            past = past[(past > c - w) | (past < sinks)]
+        rows = data["page_table"][b].long()[past // size] * size + past % size
+        keys = torch.cat([kc[rows].double() * ks, k_new[cu[b]:cu[b + 1]].double() * ks])
+        vals = torch.cat([vc[rows].double() * vs, v_new[cu[b]:cu[b + 1]].double() * vs])
+        s = torch.cat([past, torch.arange(c, c + n)])
+        here = torch.arange(c, c + n)[:, None]
+        sees = s[None, :] <= here
+        if w:
+            sees &= (s[None, :] > here - w) | (s[None, :] < sinks)
+        sc = torch.einsum("tkgd,skd->tkgs", q[cu[b]:cu[b + 1]].view(n, hkv, grp, d), keys) * cfg["sm_scale"]
+        p = torch.softmax(sc.masked_fill(~sees[:, None, None, :], -math.inf), -1)
+        out[cu[b]:cu[b + 1]] = torch.einsum("tkgs,skd->tkgd", p, vals).reshape(n, hq, d)
+    gate = x[:, (hq + 2 * hkv) * d:].view(t, hq, d)
+    out = out / torch.sqrt(out.pow(2).mean(-1, keepdim=True) + RMS_EPS) * torch.sigmoid(gate)
+    return out.reshape(t, hq * d), k_new, v_new
 
 
 def make_input(batch: int, seq_lens, seed: int, q_len: int = 1, hq: int = 32, hkv: int = 4, d: int = 128,
@@ -197,5 +256,5 @@ def to_device(data, device):
     return {k: (v.to(device) if isinstance(v, torch.Tensor) else v) for k, v in data.items()}
 
 
-__all__ = ["ref_kernel", "make_input", "rms", "rope", "quant_e4m3", "dequant_e4m3", "new_slots", "cache_rows",
+__all__ = ["ref_kernel", "ref_stream", "make_input", "rms", "rope", "quant_e4m3", "dequant_e4m3", "new_slots", "cache_rows",
            "split_qkv", "algorithmic_bytes", "to_device", "math"]
