@@ -120,6 +120,45 @@ typedef struct {
 
 int msk_attn_decode(const MskAttnParams* p, int* status, void* stream);
 
+/* ---------------------------------------------------------------- gated attention for prompts
+ * The same attention for any number of new tokens per request: request b brings the rows [cu_seqlens_q[b],
+ * cu_seqlens_q[b+1]) of qkv, its new tokens at positions seq_lens[b], seq_lens[b] + 1, ...; their keys and values are
+ * quantised and written into the pages the page table names for those positions, and attended from there.  Tokens see the
+ * positions up to their own inside the window, and the first `sinks` ones.  Requests may bring no token; rows of qkv / out
+ * outside every request are neither read nor written.  A new token whose position has no page (-1, or beyond max_pages)
+ * is reported in `status` and not written.  Reads of a page-table entry of -1 below the window and above the sinks never
+ * happen.  Stands beside msk_attn_decode, whose counterpart in the reference has only 1 or 8 new tokens per request
+ * (muse_attention_decode/submission.py:2363-2372).
+ * Built for head_dim 128, Hq = 8 * Hkv, page_size a power of two in [8, 128], sm_scale > 0.
+ */
+typedef struct {
+    const void* qkv;          /* bf16 [T, ld_qkv], rows as in MskAttnParams, 16-byte aligned */
+    int ld_qkv;               /* elements, a multiple of 8 */
+    void* out;                /* bf16 [T, ld_out] */
+    int ld_out;
+    void* k_cache;            /* as in MskAttnParams */
+    void* v_cache;
+    const float* k_scale;
+    const float* v_scale;
+    const int32_t* seq_lens;  /* [B] cached tokens per request */
+    const int32_t* cu_seqlens_q; /* [B + 1] rising, cu_seqlens_q[B] <= T */
+    const int32_t* page_table;/* [B, max_pages] */
+    int max_pages;
+    const float* inv_freq;    /* [d/2] or NULL */
+    int B, T, Hq, Hkv, d, page_size, num_pages, window, sinks;
+    float qk_scale_factor, sm_scale;
+    int splits;               /* ways the keys of a unit of 32 tokens are split over CTAs, up to 64; 0 = pick */
+    int pdl;                  /* chain the first kernel to whatever precedes it */
+    void* scratch;            /* msk_attn_prompt_scratch_bytes(), 256-byte aligned, any contents; launches that may overlap on
+                                 the GPU need one each */
+    size_t scratch_bytes;
+} MskPromptParams;
+
+int msk_attn_prompt(const MskPromptParams* p, int* status, void* stream);
+
+/* Bytes of the workspace for a call of that shape (B, T, heads, max_pages, page_size, window, sinks, splits are read). */
+int msk_attn_prompt_scratch_bytes(const MskPromptParams* p, size_t* bytes);
+
 /* ---------------------------------------------------------------- NVFP4 (w4a16) routed experts
  * Per local (token, slot) pair: h = x . W13[e]^T, inter = fp16(silu(h[:I]) * h[I:]), y = inter . W2[e]^T,
  * out[token] += topk_weight * rmsnorm(y * (1 + post_norm_w), eps); tokens without a local pair give zeros.

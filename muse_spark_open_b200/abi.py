@@ -20,7 +20,7 @@ _lib = None
 STATUS_CODES = {1: "a bounded device wait expired", 2: "an index was out of range", 3: "a work list overflowed"}
 RETURN_CODES = {-1: "invalid argument", -2: "CUDA error", -3: "unsupported shape"}
 KERNEL_NAMES = {1: "selftest", 2: "proj_skinny", 3: "attn_decode", 4: "moe_gemm1", 5: "moe_gemm2", 6: "moe_combine",
-                7: "layer_glue", 8: "ep_pack"}
+                7: "layer_glue", 8: "ep_pack", 9: "attn_prompt", 10: "pages"}
 
 
 class MskError(RuntimeError):
@@ -56,6 +56,8 @@ def lib() -> C.CDLL:
         _lib.msk_proj_skinny.argtypes = [vp, vp, vp]
         _lib.msk_proj_scratch_bytes.argtypes = [ci, ci, ci, ci, ci, vp]
         _lib.msk_attn_decode.argtypes = [vp, vp, vp]
+        _lib.msk_attn_prompt.argtypes = [vp, vp, vp]
+        _lib.msk_attn_prompt_scratch_bytes.argtypes = [vp, vp]
         _lib.msk_moe_packed_bytes.argtypes = [ci, ci, ci, vp, vp]
         _lib.msk_moe_pack.argtypes = [vp, vp, vp, vp]
         _lib.msk_moe_dequant.argtypes = [vp, vp, ci, ci, ci, ci, vp]
@@ -82,6 +84,7 @@ def lib() -> C.CDLL:
 
 # every symbol include/msk.h declares
 EXPORTS = ["msk_version", "msk_device_info", "msk_selftest_umma", "msk_proj_skinny", "msk_proj_scratch_bytes", "msk_attn_decode",
+           "msk_attn_prompt", "msk_attn_prompt_scratch_bytes",
            "msk_moe_packed_bytes", "msk_moe_pack", "msk_moe_dequant", "msk_moe_scratch_bytes", "msk_moe_forward", "msk_moe_forward_static", "msk_layer_front", "msk_layer_decode", "msk_router", "msk_residual_boundary", "msk_rmsnorm",
            "msk_ep_row_bytes", "msk_ep_pack", "msk_ep_reduce", "msk_ep_region_bytes", "msk_ep_region_alloc", "msk_ep_region_open",
            "msk_ep_region_close", "msk_ep_region_free", "msk_ep_step", "msk_selftest_flag_timeout"]
@@ -145,6 +148,19 @@ class AttnParams(C.Structure):
         ("qk_scale_factor", C.c_float), ("sm_scale", C.c_float),
         ("chunks", C.c_int), ("stages", C.c_int), ("issuers", C.c_int), ("pdl", C.c_int), ("row_groups", C.c_int),
         ("sinks", C.c_int),
+    ]
+
+
+class PromptParams(C.Structure):
+    _fields_ = [
+        ("qkv", C.c_void_p), ("ld_qkv", C.c_int), ("out", C.c_void_p), ("ld_out", C.c_int),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("seq_lens", C.c_void_p), ("cu_seqlens_q", C.c_void_p), ("page_table", C.c_void_p), ("max_pages", C.c_int),
+        ("inv_freq", C.c_void_p),
+        ("B", C.c_int), ("T", C.c_int), ("Hq", C.c_int), ("Hkv", C.c_int), ("d", C.c_int), ("page_size", C.c_int),
+        ("num_pages", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
+        ("qk_scale_factor", C.c_float), ("sm_scale", C.c_float), ("splits", C.c_int), ("pdl", C.c_int),
+        ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
     ]
 
 

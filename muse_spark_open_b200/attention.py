@@ -62,3 +62,47 @@ def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
     out = torch.empty((b, l, hq * d), dtype=torch.bfloat16, device=qkv.device)
     launch(qkv.view(b * l, -1), out.view(b * l, hq * d), data, cfg, chunks, stages)
     return out
+
+
+def prompt_fn(data: dict, out: torch.Tensor | None = None, splits: int = 0) -> torch.Tensor:
+    """bf16 [T, Hq*d]: the same attention for prompts, with any number of new tokens per request.
+
+    `data` as for `kernel_fn`, except: qkv is [T, (2Hq+2Hkv)*d] (row stride free), cu_seqlens_q int32 [B + 1] says which
+    rows belong to which request, and there is no cache_loc (the rows of the new K/V follow from the page table, whose
+    entries must exist for the new positions: `pages.extend`).  `config` needs no q_len.  Rows behind cu_seqlens_q[B]
+    (a padded batch) are not touched: they keep what `out` held.  The workspace comes from torch's allocator on the current
+    stream, so calls on several streams or in several captured graphs do not share it.
+    """
+    cfg, qkv, kc, vc = data["config"], data["qkv"], data["k_cache"], data["v_cache"]
+    table, seq, cu = data["page_table"], data["seq_lens"], data["cu_seqlens_q"]
+    b, hq, hkv, d = cfg["batch"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"]
+    if qkv.dtype != torch.bfloat16 or kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
+        raise abi.MskError("qkv must be bfloat16 and the cache float8_e4m3fn")
+    if qkv.dim() != 2 or qkv.shape[1] < (2 * hq + 2 * hkv) * d or qkv.stride(1) != 1:
+        raise abi.MskError("qkv must be [tokens, (2Hq+2Hkv)*d] with unit column stride")
+    if seq.dtype != torch.int32 or table.dtype != torch.int32 or cu.dtype != torch.int32:
+        raise abi.MskError("seq_lens / page_table / cu_seqlens_q must be int32")
+    if seq.numel() != b or table.dim() != 2 or table.shape[0] != b or cu.numel() != b + 1 or \
+            not (seq.is_contiguous() and table.is_contiguous() and cu.is_contiguous()):
+        raise abi.MskError("seq_lens [B], page_table [B, max_pages] and cu_seqlens_q [B + 1] must be contiguous")
+    shape = (kc.shape[0], cfg["page_size"], hkv, d)
+    if kc.shape != shape or vc.shape != shape or not (kc.is_contiguous() and vc.is_contiguous()):
+        raise abi.MskError("k_cache / v_cache must be contiguous [num_pages, page_size, Hkv, d]")
+    t, dev = qkv.shape[0], qkv.device
+    if out is None:
+        out = torch.empty((t, hq * d), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.shape != (t, hq * d) or out.stride(1) != 1:
+        raise abi.MskError("out must be bfloat16 [tokens, Hq*d] with unit column stride")
+    if t == 0:
+        return out
+    f = inv_freq(cfg["rope_theta"], d, dev)
+    p = abi.PromptParams(
+        abi.ptr(qkv), qkv.stride(0), abi.ptr(out), out.stride(0), abi.ptr(kc), abi.ptr(vc), abi.ptr(data["k_scale"]), abi.ptr(data["v_scale"]),
+        abi.ptr(seq), abi.ptr(cu), abi.ptr(table), table.shape[1], abi.ptr(f), b, t, hq, hkv, d, cfg["page_size"], kc.shape[0],
+        cfg["window"], cfg.get("sinks", 0), cfg["qk_scale_factor"], cfg["sm_scale"], splits, 0, None, 0)
+    lib, n = abi.lib(), C.c_size_t()
+    abi.check(lib.msk_attn_prompt_scratch_bytes(C.byref(p), C.byref(n)), "msk_attn_prompt_scratch_bytes")
+    scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    p.scratch, p.scratch_bytes = scratch.data_ptr(), n.value
+    abi.check(lib.msk_attn_prompt(C.byref(p), abi.status_for(dev).p, abi.stream_ptr()), "msk_attn_prompt")
+    return out

@@ -44,8 +44,7 @@
 // position t when s <= t and (s > t - window or s < sinks).  Only the tiles that hold such keys are read (the pages in
 // between may be gone: table entry -1), so a long context costs window + sinks keys.
 // Roofline: HBM (K and V bytes of the visible keys, read once).
-#include <cuda_fp8.h>
-
+#include "attn_common.cuh"
 #include "msk.h"
 #include "ptx.cuh"
 #include "tmap.cuh"
@@ -78,34 +77,6 @@ struct AttnArgs {
     float qk_scale_factor, sm_scale, q_split_scale;
     int* status;
 };
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float redux_max(float v) {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
-__device__ __forceinline__ uint32_t f2_to_e4m3x2(float a, float b) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ float e4m3_to_f(uint32_t byte) {
-    __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3);
-    return __half2float(*reinterpret_cast<__half*>(&h));
-}
-__device__ __forceinline__ float2 e4m3x2_to_f2(uint32_t two) {  // low byte -> x
-    __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-    return __half22float2(*reinterpret_cast<__half2*>(&h));
-}
-__device__ __forceinline__ uint32_t f_to_e4m3(float a) {
-    return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ uint32_t f_to_e5m2(float a) {
-    return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E5M2);
-}
 
 // RMSNorm (weightless, eps 1e-5) and interleaved RoPE of one 128-wide head row held 4 values per lane.
 __device__ __forceinline__ void norm_rope_row(float (&x)[4], float post_scale, const float* inv_freq, int pos, int lane) {

@@ -1,0 +1,736 @@
+// Gated attention for prompts: any number of new tokens per request behind any number of cached ones, over the paged
+// FP8-E4M3 cache, with a sliding window and first tokens that stay visible.  Two launches, three when the keys are split:
+//
+//   prep     one CTA per token: RMSNorm, scale and RoPE of its queries (rounded to BF16, kept as FP16 in the workspace) and
+//            keys; keys and values quantised to E4M3 and written into the pages the page table names.  One more CTA lists
+//            the work units (request, first token).  Bound by memory: 18 KB per token at 32 + 4 + 4 heads.
+//   main     one CTA per (unit of 32 new tokens, KV head, split): flash attention.  The 8 query heads of a KV head and the
+//            tokens together are the rows of the product: 2 tiles of 128 rows = 16 tokens x 8 heads.
+//   combine  one warp per (token, head): joins the splits' (m, l, O); used when there are fewer units than SMs.
+//
+// Main kernel, per 128-key tile (FP16 tensor-core operands: E4M3 cache values and BF16 queries are exact in FP16, and
+// FP16 probabilities are off by 2^-12, so the result carries little more than its last rounding):
+//   copying warp     TMA boxes of the K and V pages into 2 x 16 KB of E4M3 staging
+//   converting warps E4M3 -> FP16 into the swizzled operand tiles (two slots each for K and V), rows no token sees as zeros
+//   MMA thread       S = Q K^T into TMEM (128 x 128 FP32 per row tile), O += P V with P from TMEM
+//   softmax warps    thread = row: the row's 128 scores come from TMEM in one go, no shuffles; p = 2^(s - m) goes back as
+//                    FP16 over the scores.  The running reference m moves only when a row's maximum outgrows it by 2^8,
+//                    so the accumulator in TMEM is rescaled a few times per row, not once per tile.
+// The two row tiles take turns: while one's scores are exponentiated, the tensor cores work on the other's products.
+// TMEM: S (with P over its first half) and O, 128 columns each, for two row tiles = all 512 columns.
+#include "attn_common.cuh"
+#include "msk.h"
+#include "ptx.cuh"
+#include "tmap.cuh"
+
+namespace msk {
+namespace {
+
+constexpr int kTile = 128;                  // keys per tile
+constexpr int kTok = 16;                    // tokens per row tile
+constexpr int kUnitTok = 2 * kTok;          // tokens per unit
+constexpr int kThreads = 512;               // softmax A | softmax B | converting | MMA, copying, two idle warps
+constexpr int kQBytes = 32768;              // one row tile of queries: two swizzled halves of 64 channels
+constexpr int kF16Tile = 32768;             // one K or V tile as FP16
+constexpr int kF8Tile = 16384;
+constexpr int kSmem = 2 * kQBytes + 4 * kF16Tile + 2 * kF8Tile + 1024;
+constexpr float kNegRef = -1.0e30f;
+constexpr float kLazy = 8.0f;               // how far (in powers of two) a row's maximum may outgrow its reference
+constexpr int kMaxUnitsHeader = 4;          // ints before the unit list: their number, padding
+
+struct PromptArgs {
+    const __nv_bfloat16* qkv;
+    int ld_qkv;
+    __nv_bfloat16* out;
+    int ld_out;
+    uint8_t* k_cache;
+    uint8_t* v_cache;
+    const float* k_scale;
+    const float* v_scale;
+    const int* seq_lens;
+    const int* cu;
+    const int* page_table;
+    int max_pages;
+    const float* inv_freq;
+    int B, T, Hq, Hkv, page_size, page_log, num_pages, window, sinks, splits, max_units;
+    float qk_scale_factor, q_scale, s_scale;  // queries are stored times q_scale (a power of two); scores times s_scale * k_scale
+    __half* q16;      // [T, Hq, 128]
+    int* units;       // [kMaxUnitsHeader + 2 * max_units]
+    float* part_o;    // [splits, T * Hq, 128]
+    float* part_ml;   // [splits, T * Hq, 2]
+    int* status;
+};
+
+__device__ __forceinline__ int new_tokens(const PromptArgs& p, int b) {
+    const int lo = min(max(p.cu[b], 0), p.T), hi = min(max(p.cu[b + 1], 0), p.T);
+    return max(hi - lo, 0);
+}
+
+// RMSNorm (weightless, eps 1e-5), scale and interleaved RoPE of one 128-wide head row, 4 values per lane.
+__device__ __forceinline__ void norm_turn(float (&x)[4], float post_scale, const float (&c)[2], const float (&s)[2], bool turn) {
+    float ss = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
+    ss = warp_sum(ss);
+    const float r = 1.0f / sqrtf(ss * (1.0f / 128.0f) + 1e-5f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (x[i] * r) * post_scale;
+    if (turn) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float e = x[2 * h], o = x[2 * h + 1];
+            x[2 * h] = e * c[h] - o * s[h];
+            x[2 * h + 1] = e * s[h] + o * c[h];
+        }
+    }
+}
+
+// The unit list: for each request its groups of 32 new tokens, the last group first (it sees the most keys, so the long
+// units start early).  One CTA.
+__device__ void list_units(const PromptArgs& p) {
+    __shared__ int carry_s, warp_s[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) carry_s = 0;
+    __syncthreads();
+    for (int b0 = 0; b0 < p.B; b0 += 256) {
+        const int b = b0 + tid;
+        const int n = b < p.B ? new_tokens(p, b) : 0;
+        const int tiles = (n + kUnitTok - 1) / kUnitTok;
+        int inc = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) warp_s[warp] = inc;
+        __syncthreads();
+        int before = carry_s, total = 0;
+        for (int w = 0; w < 8; ++w) {
+            if (w < warp) before += warp_s[w];
+            total += warp_s[w];
+        }
+        const int at = before + inc - tiles;
+        for (int i = 0; i < tiles; ++i) {
+            if (at + i < p.max_units) {
+                p.units[kMaxUnitsHeader + 2 * (at + i)] = b;
+                p.units[kMaxUnitsHeader + 2 * (at + i) + 1] = (tiles - 1 - i) * kUnitTok;
+            }
+        }
+        __syncthreads();
+        if (tid == 0) carry_s += total;
+        __syncthreads();
+    }
+    if (tid == 0) {
+        if (carry_s > p.max_units) report(p.status, MSK_ERR_CAPACITY, MSK_K_PROMPT << 8 | 1, carry_s, p.max_units);
+        p.units[0] = min(carry_s, p.max_units);
+    }
+}
+
+__global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int t = blockIdx.x;
+    if (t == p.T) {
+        list_units(p);
+        return;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // the request of token t: the last b with cu[b] <= t, by steps of 32 requests
+    int lo = 0, hi = p.B;  // cu[lo] <= t < cu[hi] is looked for in [lo, hi)
+    if (t >= p.cu[p.B] || t < p.cu[0]) return;  // a row behind the last sequence
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + step * lane;
+        const bool le = at < hi && p.cu[at] <= t;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, le) | 1u);
+        const int nlo = lo + step * k;
+        hi = min(hi, nlo + step);
+        lo = nlo;
+    }
+    const int b = lo;
+    const int pos = p.seq_lens[b] + t - p.cu[b];
+    float c[2] = {1.0f, 1.0f}, s[2] = {0.0f, 0.0f};
+    const bool turn = p.inv_freq != nullptr;
+    if (turn) {
+        const float fp = static_cast<float>(pos);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // the product's rounding error (up to 5e-4 at position 8192) is put back to first order
+            const float f = p.inv_freq[2 * lane + h], ang = fp * f, err = fmaf(fp, f, -ang);
+            float cs, sn;
+            sincosf(ang, &sn, &cs);
+            c[h] = cs - err * sn;
+            s[h] = sn + err * cs;
+        }
+    }
+    const __nv_bfloat16* row = p.qkv + static_cast<size_t>(t) * p.ld_qkv;
+    const int heads = p.Hq + 2 * p.Hkv;
+    const int page = pos >> p.page_log;
+    const int id = pos >= 0 && page < p.max_pages ? p.page_table[static_cast<size_t>(b) * p.max_pages + page] : -1;
+    const bool page_ok = id >= 0 && id < p.num_pages;
+    if (!page_ok && threadIdx.x == 0) report(p.status, MSK_ERR_BOUNDS, MSK_K_PROMPT << 8 | 2, id, page);
+    const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
+    const size_t slot = page_ok ? (static_cast<size_t>(id) << p.page_log) + (pos & (p.page_size - 1)) : 0;
+    constexpr int U = 5;  // rows in flight per warp: 8 warps cover 40 heads at once
+    for (int h0 = warp; h0 < heads; h0 += 8 * U) {
+        uint2 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (h0 + 8 * u < heads) raw[u] = *reinterpret_cast<const uint2*>(row + (h0 + 8 * u) * 128 + 4 * lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + 8 * u;
+            if (h >= heads) break;
+            float x[4] = {bf16lo(raw[u].x), bf16hi(raw[u].x), bf16lo(raw[u].y), bf16hi(raw[u].y)};
+            if (h < p.Hq) {
+                norm_turn(x, p.qk_scale_factor, c, s, turn);
+                __half2 a[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    a[i] = __floats2half2_rn(__bfloat162float(__float2bfloat16(x[2 * i])) * p.q_scale,
+                                             __bfloat162float(__float2bfloat16(x[2 * i + 1])) * p.q_scale);
+                *reinterpret_cast<uint2*>(p.q16 + (static_cast<size_t>(t) * p.Hq + h) * 128 + 4 * lane) =
+                    make_uint2(*reinterpret_cast<uint32_t*>(&a[0]), *reinterpret_cast<uint32_t*>(&a[1]));
+            } else {
+                const bool key = h < p.Hq + p.Hkv;
+                if (key) norm_turn(x, 1.0f, c, s, turn);
+                const float sc = key ? k_scale : v_scale;
+                const uint32_t w = f2_to_e4m3x2(__fdiv_rn(x[0], sc), __fdiv_rn(x[1], sc)) |
+                                   f2_to_e4m3x2(__fdiv_rn(x[2], sc), __fdiv_rn(x[3], sc)) << 16;
+                const int kv = h - p.Hq - (key ? 0 : p.Hkv);
+                if (page_ok)
+                    *reinterpret_cast<uint32_t*>((key ? p.k_cache : p.v_cache) + (slot * p.Hkv + kv) * 128 + 4 * lane) = w;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t low_bits(int n) {  // bits [0, n) set, n clamped to [0, 32]
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// The last steps for one row held by one thread: value = o * inv, RMSNorm over 128 channels, sigmoid gate, BF16.
+// `load`: the 32 values of chunk c.
+template <class Load>
+__device__ __forceinline__ void finish_row(const PromptArgs& p, Load load, float inv, bool live, size_t token, int head) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        load(c, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float o = __uint_as_float(v[i]) * inv;
+            ss += o * o;
+        }
+    }
+    const float r = inv / sqrtf(ss * (1.0f / 128.0f) + 1e-5f);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint4 g[4];
+        const __nv_bfloat16* gate = p.qkv + token * p.ld_qkv + (p.Hq + 2 * p.Hkv + head) * 128 + 32 * c;
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) g[i] = *reinterpret_cast<const uint4*>(gate + 8 * i);
+        }
+        uint32_t v[32];
+        load(c, v);
+        if (live) {
+            __nv_bfloat16* dst = p.out + token * p.ld_out + head * 128 + 32 * c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float a = __uint_as_float(v[8 * i + 2 * j]) * r / (1.0f + __expf(-bf16lo(gw[j])));
+                    const float b = __uint_as_float(v[8 * i + 2 * j + 1]) * r / (1.0f + __expf(-bf16hi(gw[j])));
+                    w[j] = pack_bf16(a, b);
+                }
+                *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, PromptArgs p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[20];
+    __shared__ uint32_t tmem_slot;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int h = blockIdx.x % p.Hkv, sp = (blockIdx.x / p.Hkv) % p.splits, slot_u = blockIdx.x / (p.Hkv * p.splits);
+    const int where = MSK_K_PROMPT << 8;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t s_q = base, s_k = s_q + 2 * kQBytes, s_v = s_k + 2 * kF16Tile, s_f8 = s_v + 2 * kF16Tile;
+    uint8_t* g_k = gbase + 2 * kQBytes;
+    uint8_t* g_v = g_k + 2 * kF16Tile;
+    uint8_t* g_f8 = g_v + 2 * kF16Tile;
+    auto bar = [&](int i) { return smem_u32(&bars[i]); };
+    // staging full / free (K, V); operand slots full / free; queries; scores, P per row tile; output
+    const uint32_t st_full = bar(0), st_free = bar(2), k_full = bar(4), k_free = bar(6), v_full = bar(8), v_free = bar(10),
+                   q_full = bar(12), s_done = bar(14), p_ready = bar(16), o_done = bar(18);
+
+    if (warp == 0) {
+        tmem_alloc(smem_u32(&tmem_slot), 512);
+        tmem_relinquish();
+    }
+    if (tid == 32) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(st_full + 8 * i, 1), mbar_init(st_free + 8 * i, 4);
+            mbar_init(k_full + 8 * i, 4), mbar_init(k_free + 8 * i, 1);
+            mbar_init(v_full + 8 * i, 4), mbar_init(v_free + 8 * i, 1);
+            mbar_init(s_done + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(o_done, 1);
+        fence_mbar_init();
+    }
+    if (tid == 64) prefetch_tmap(&tm_q), prefetch_tmap(&tm_k), prefetch_tmap(&tm_v);
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---------------- this CTA's unit
+    const int n_units = p.units[0];
+    const bool have = slot_u < n_units;
+    const int b = have ? p.units[kMaxUnitsHeader + 2 * slot_u] : 0;
+    const int q0 = have ? p.units[kMaxUnitsHeader + 2 * slot_u + 1] : 0;
+    const int tok0 = min(max(p.cu[b], 0), p.T) + q0;       // first row of qkv / out
+    const int n_tok = have ? min(new_tokens(p, b) - q0, kUnitTok) : 0;
+    const int p_first = p.seq_lens[b] + q0, p_last = p_first + max(n_tok, 1) - 1;
+    const int W = p.window, snk = W > 0 ? p.sinks : 0;
+    const int t_first = (W > 0 ? max(0, p_first - W + 1) : 0) / kTile;
+    const int sink_tiles = min((min(snk, p_last + 1) + kTile - 1) / kTile, t_first);
+    const int gap = t_first - sink_tiles;
+    const int tiles = have ? p_last / kTile - t_first + 1 + sink_tiles : 0;
+    const int per = (tiles + p.splits - 1) / p.splits;
+    const int v_begin = sp * per;
+    const int nt = max(0, min(per, tiles - v_begin));
+    const bool two = n_tok > kTok;                         // the second row tile has tokens
+    auto base_of = [&](int i) { return (v_begin + i + (v_begin + i >= sink_tiles ? gap : 0)) * kTile; };
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
+
+    if (warp < 8) {
+        // ================ softmax: thread = row of row tile g
+        reg_inc<192>();
+        const int g = warp >> 2, row = tid & 127, j = row >> 3, head = h * 8 + (row & 7);
+        const int pos = p_first + g * kTok + j;
+        const bool live = g * kTok + j < n_tok;
+        const size_t token = static_cast<size_t>(tok0) + g * kTok + j;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
+        const float scale = k_scale * p.s_scale;
+        const int g_first = p_first + g * kTok, g_last = g_first + kTok - 1;
+        float m = kNegRef, l = 0.0f;
+        bool ok = true;
+        if (g == 0 || two) {
+            for (int i = 0; i < nt; ++i) {
+                ok = mbar_wait(s_done + 8 * g, i & 1, p.status, where | 3) && ok;
+                tc_fence_after();
+                const int s0 = base_of(i);
+                uint32_t x[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x[c]);
+                tmem_wait_ld();
+                if (s0 + kTile - 1 > g_first || (W > 0 && s0 <= g_last - W && s0 + kTile > snk)) {
+                    // an edge of what the rows see: one bit per key
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int at = s0 + 32 * c;
+                        uint32_t vis = low_bits(pos - at + 1);
+                        if (W > 0) vis &= ~low_bits(pos - W - at + 1) | low_bits(snk - at);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(vis & (1u << e))) x[c][e] = 0xff800000u;  // -inf
+                    }
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    mx[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+                    for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][e]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // the reference moves when the maximum has outgrown it by 2^kLazy (p then stays below 2^8 in FP16)
+                const bool move = (top - m) * scale > kLazy;
+                const float m_new = move ? top : m;
+                const float alpha = move ? ex2((m - m_new) * scale) : 1.0f;
+                const bool any = __any_sync(0xffffffffu, move);
+                m = m_new;
+                const float off = -m * scale;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; c += 2) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int cc = c + (e >> 4), k = 2 * (e & 15);
+                        const float a = ex2(fmaf(__uint_as_float(x[cc][k]), scale, off));
+                        const float bb = ex2(fmaf(__uint_as_float(x[cc][k + 1]), scale, off));
+                        sum[(e & 1) * 2] += a;
+                        sum[(e & 1) * 2 + 1] += bb;
+                        w[e] = pack_half(a, bb);
+                    }
+                    tmem_st32(t_s + 16 * c, w);
+                }
+                l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                if (any && i > 0) {  // the accumulator follows the reference (its last product is done: S came after it)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + 32 * c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(t_o + 32 * c, o);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready + 8 * g);
+            }
+            if (nt > 0) {
+                ok = mbar_wait(o_done, 0, p.status, where | 4) && ok;
+                ok = __all_sync(0xffffffffu, ok);
+                tc_fence_after();
+            }
+            auto load = [&](int c, uint32_t (&v)[32]) {
+                tmem_ld32(t_o + 32 * c, v);
+                tmem_wait_ld();
+            };
+            if (p.splits == 1) {
+                if (nt > 0 && ok) finish_row(p, load, v_scale / l, live, token, head);
+            } else {
+                const size_t r = (static_cast<size_t>(sp) * p.T + token) * p.Hq + head;
+                if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(nt > 0 && ok ? m * scale : kNegRef, nt > 0 && ok ? l : 0.0f);
+                if (nt > 0) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        load(c, v);
+                        if (live) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                *reinterpret_cast<uint4*>(p.part_o + r * 128 + 32 * c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ================ converting: E4M3 staging -> FP16 operand tiles
+        reg_dec<64>();
+        const int w = warp - 8;
+        bool ok = true;
+        for (int i = 0; i < nt && ok; ++i) {
+            const int s0 = base_of(i), slot = i & 1;
+#pragma unroll 1
+            for (int kv = 0; kv < 2; ++kv) {
+                ok = mbar_wait(st_full + 8 * kv, i & 1, p.status, where | 5) && ok;
+                if (i >= 2) ok = mbar_wait((kv ? v_free : k_free) + 8 * slot, ((i >> 1) - 1) & 1, p.status, where | 6) && ok;
+                if (!ok) break;
+                const uint8_t* src = g_f8 + kv * kF8Tile;
+                uint8_t* dst = (kv ? g_v : g_k) + slot * kF16Tile;
+                // 8 lanes cover 64 bytes of row r and the other 64 of row r + 1: 16-byte loads and stores without conflicts
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int r = w * 32 + (u >> 1) * 8 + (lane >> 2);
+                    const int c = (lane & 3) + 4 * (((lane >> 2) ^ u) & 1);
+                    uint4 in = *reinterpret_cast<const uint4*>(src + r * 128 + c * 16);
+                    if (kv) {
+                        // values no token sees may be anything (even NaN): zeros, so that 0 * V stays 0
+                        const int pos = s0 + r;
+                        if (pos > p_last || (W > 0 && pos <= p_first - W && pos >= snk)) in = make_uint4(0, 0, 0, 0);
+                    }
+                    const uint32_t q[4] = {in.x, in.y, in.z, in.w};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[e]), __NV_E4M3);
+                        const __half2_raw d = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[e] >> 16), __NV_E4M3);
+                        o[2 * e] = *reinterpret_cast<const uint32_t*>(&a);
+                        o[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&d);
+                    }
+                    uint8_t* half = dst + (c >> 2) * 16384;
+                    *reinterpret_cast<uint4*>(half + swz128(r, (c & 3) * 32)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(half + swz128(r, (c & 3) * 32 + 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(st_free + 8 * kv);
+                    mbar_arrive((kv ? v_full : k_full) + 8 * slot);
+                }
+            }
+        }
+    } else {
+        reg_dec<64>();
+        if (warp == 12) {
+            // ================ the MMA thread
+            if (lane == 0 && nt > 0) {
+                const uint32_t id_qk = umma_idesc(128, 128, 0, 0, 0, 0), id_pv = umma_idesc(128, 128, 0, 0, 0, 1);
+                auto scores = [&](int g, int slot) {  // S_g = Q_g K^T
+                    const uint64_t a = umma_smem_desc(s_q + g * kQBytes, 16, 1024, kSwizzle128);
+                    const uint64_t k = umma_smem_desc(s_k + slot * kF16Tile, 16, 1024, kSwizzle128);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t o = ((e >> 2) * 16384 + (e & 3) * 32) >> 4;
+                        umma_f16_ss(tmem + g * 128, a + o, k + o, id_qk, e != 0);
+                    }
+                    umma_commit(s_done + 8 * g);
+                };
+                auto output = [&](int g, int slot, bool first) {  // O_g (+)= P_g V
+                    const uint64_t v = umma_smem_desc(s_v + slot * kF16Tile, 16384, 1024, kSwizzle128);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + 8 * e, v + ((2048 * e) >> 4), id_pv, !first || e != 0);
+                };
+                bool ok = mbar_wait(q_full, 0, p.status, where | 7) && mbar_wait(k_full, 0, p.status, where | 8);
+                if (ok) {
+                    tc_fence_after();
+                    scores(0, 0);
+                    if (two) scores(1, 0);
+                    umma_commit(k_free);
+                }
+                for (int i = 0; i < nt && ok; ++i) {
+                    const int slot = i & 1, nslot = slot ^ 1;
+                    ok = mbar_wait(v_full + 8 * slot, (i >> 1) & 1, p.status, where | 9) && mbar_wait(p_ready, i & 1, p.status, where | 10);
+                    if (!ok) break;
+                    tc_fence_after();
+                    output(0, slot, i == 0);
+                    const bool more = i + 1 < nt;
+                    if (more) {
+                        ok = mbar_wait(k_full + 8 * nslot, ((i + 1) >> 1) & 1, p.status, where | 11);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(0, nslot);
+                    }
+                    if (two) {
+                        ok = mbar_wait(p_ready + 8, i & 1, p.status, where | 12);
+                        if (!ok) break;
+                        tc_fence_after();
+                        output(1, slot, i == 0);
+                    }
+                    umma_commit(v_free + 8 * slot);
+                    if (more) {
+                        if (two) scores(1, nslot);
+                        umma_commit(k_free + 8 * nslot);
+                    }
+                }
+                umma_commit(o_done);
+            }
+            __syncwarp();
+        } else if (warp == 13 && nt > 0) {
+            // ================ the copying warp
+            if (lane == 0) {
+                mbar_expect_tx(q_full, (two ? 2 : 1) * kQBytes);
+                for (int g = 0; g < (two ? 2 : 1); ++g)
+                    for (int c = 0; c < 2; ++c)
+                        tma_load_3d(s_q + g * kQBytes + c * 16384, &tm_q, q_full, 64 * c, h * 8, tok0 + g * kTok);
+            }
+            const int ppt = kTile >> p.page_log;  // pages per tile, <= 16: lane j fetches page j
+            auto page_of = [&](int i) {
+                const int pg = (base_of(i) >> p.page_log) + lane;
+                int id = lane < ppt && pg < p.max_pages ? p.page_table[static_cast<size_t>(b) * p.max_pages + pg] : -1;
+                if (id >= p.num_pages || id < -1) {
+                    report(p.status, MSK_ERR_BOUNDS, where | 13, id, p.num_pages);
+                    id = -1;
+                }
+                return id;  // -1: zeros
+            };
+            int id = page_of(0);
+            bool ok = true;
+            for (int i = 0; i < nt && ok; ++i) {
+                const int next = i + 1 < nt ? page_of(i + 1) : -1;
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (i > 0) ok = mbar_wait(st_free + 8 * kv, (i - 1) & 1, p.status, where | 14) && ok;
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(st_full + 8 * kv, kF8Tile);
+                    __syncwarp();
+                    if (lane < ppt)
+                        tma_load_4d(s_f8 + kv * kF8Tile + (lane << p.page_log) * 128, kv ? &tm_v : &tm_k, st_full + 8 * kv, 0, h, 0, id);
+                }
+                id = next;
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// Joins the splits of one (token, head) per warp: lane = 4 channels.
+__global__ void __launch_bounds__(256) prompt_combine_kernel(PromptArgs p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int token = static_cast<int>(row / p.Hq), head = static_cast<int>(row % p.Hq);
+    const int last = min(p.cu[p.B], p.T);
+    if (token >= last || token < p.cu[0]) return;
+    const size_t stride = static_cast<size_t>(p.T) * p.Hq;
+    float m = kNegRef;
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (s * stride + row)]);
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < p.splits; ++s) {
+        const size_t r = s * stride + row;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * r);
+        if (ml.y > 0.0f) {  // a split without keys has written no output
+            const float w = ex2(ml.x - m);
+            const float4 v = *reinterpret_cast<const float4*>(p.part_o + r * 128 + 4 * lane);
+            l += w * ml.y;
+            o[0] += w * v.x, o[1] += w * v.y, o[2] += w * v.z, o[3] += w * v.w;
+        }
+    }
+    const float inv = l > 0.0f ? __ldg(p.v_scale) / l : 0.0f;
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= inv, ss += o[i] * o[i];
+    ss = warp_sum(ss);
+    const float r = 1.0f / sqrtf(ss * (1.0f / 128.0f) + 1e-5f);
+    const uint2 g = *reinterpret_cast<const uint2*>(p.qkv + static_cast<size_t>(token) * p.ld_qkv + (p.Hq + 2 * p.Hkv + head) * 128 + 4 * lane);
+    const float gate[4] = {bf16lo(g.x), bf16hi(g.x), bf16lo(g.y), bf16hi(g.y)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = o[i] * r / (1.0f + __expf(-gate[i]));
+    *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(token) * p.ld_out + head * 128 + 4 * lane) =
+        make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+}
+
+struct Plan {
+    int max_units, splits;
+    size_t q16, units, ml, o, total;  // byte offsets, and the end
+};
+
+int plan_prompt(const MskPromptParams* q, Plan* plan) {
+    if (q->d != 128 || q->Hkv < 1 || q->Hq != 8 * q->Hkv || q->B < 1 || q->T < 1 || q->max_pages < 1) return MSK_ERR_UNSUPPORTED;
+    if (q->page_size < 8 || q->page_size > 128 || (q->page_size & (q->page_size - 1)) != 0) return MSK_ERR_UNSUPPORTED;
+    if (q->window < 0 || q->sinks < 0 || q->splits < 0 || q->splits > 64) return MSK_ERR_INVALID;
+    const long long units = static_cast<long long>(q->T) / kUnitTok + q->B;  // sum of ceil(n / 32) is at most this
+    plan->max_units = static_cast<int>(units < q->T ? units : q->T);
+    long long tiles = (static_cast<long long>(q->max_pages) * q->page_size + kTile - 1) / kTile;
+    if (q->window > 0) {
+        const long long w = static_cast<long long>(q->window + kUnitTok) / kTile + 2 + (q->sinks + kTile - 1) / kTile;
+        if (w < tiles) tiles = w;
+    }
+    plan->splits = q->splits;
+    if (q->splits == 0) {
+        // fewer units than SMs: the keys are split, down to two tiles a piece
+        const long long ctas = static_cast<long long>(plan->max_units) * q->Hkv;
+        long long s = 148 / ctas;
+        if (s > (tiles + 1) / 2) s = (tiles + 1) / 2;
+        if (s > 32) s = 32;
+        plan->splits = s < 1 ? 1 : static_cast<int>(s);
+    }
+    auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
+    const size_t rows = static_cast<size_t>(q->T) * q->Hq;
+    plan->q16 = 0;
+    plan->units = up(rows * 256);
+    plan->ml = plan->units + up((kMaxUnitsHeader + 2 * static_cast<size_t>(plan->max_units)) * 4);
+    const size_t parts = plan->splits > 1 ? static_cast<size_t>(plan->splits) * rows : 0;
+    plan->o = plan->ml + up(parts * 8);
+    plan->total = plan->o + up(parts * 512);
+    return 0;
+}
+
+}  // namespace
+}  // namespace msk
+
+extern "C" int msk_attn_prompt_scratch_bytes(const MskPromptParams* q, size_t* bytes) {
+    msk::Plan plan;
+    if (q == nullptr || bytes == nullptr) return MSK_ERR_INVALID;
+    const int rc = msk::plan_prompt(q, &plan);
+    if (rc == 0) *bytes = plan.total;
+    return rc;
+}
+
+extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stream) {
+    using namespace msk;
+    if (q == nullptr || !q->qkv || !q->out || !q->k_cache || !q->v_cache || !q->k_scale || !q->v_scale || !q->seq_lens ||
+        !q->cu_seqlens_q || !q->page_table || !q->scratch)
+        return MSK_ERR_INVALID;
+    Plan plan;
+    int rc = plan_prompt(q, &plan);
+    if (rc != 0) return rc;
+    const int wide = (2 * q->Hq + 2 * q->Hkv) * 128;
+    if (q->scratch_bytes < plan.total || (reinterpret_cast<uintptr_t>(q->scratch) & 255) != 0) return MSK_ERR_INVALID;
+    if (q->ld_qkv < wide || q->ld_out < q->Hq * 128 || q->ld_qkv % 8 != 0 || q->ld_out % 8 != 0) return MSK_ERR_INVALID;
+    if (((reinterpret_cast<uintptr_t>(q->qkv) | reinterpret_cast<uintptr_t>(q->out) | reinterpret_cast<uintptr_t>(q->k_cache) |
+          reinterpret_cast<uintptr_t>(q->v_cache)) & 15) != 0)
+        return MSK_ERR_INVALID;
+    if (!(q->sm_scale > 0.0f) || !(q->sm_scale < 1e30f)) return MSK_ERR_INVALID;
+    const long long ctas = static_cast<long long>(plan.max_units) * plan.splits * q->Hkv;
+    if (ctas > 0x7fffffffll || static_cast<long long>(q->T) * q->Hq > 0x7fffffffll) return MSK_ERR_UNSUPPORTED;
+
+    uint8_t* ws = static_cast<uint8_t*>(q->scratch);
+    PromptArgs a{};
+    a.qkv = static_cast<const __nv_bfloat16*>(q->qkv), a.ld_qkv = q->ld_qkv;
+    a.out = static_cast<__nv_bfloat16*>(q->out), a.ld_out = q->ld_out;
+    a.k_cache = static_cast<uint8_t*>(q->k_cache), a.v_cache = static_cast<uint8_t*>(q->v_cache);
+    a.k_scale = q->k_scale, a.v_scale = q->v_scale, a.seq_lens = q->seq_lens, a.cu = q->cu_seqlens_q;
+    a.page_table = q->page_table, a.max_pages = q->max_pages, a.inv_freq = q->inv_freq;
+    a.B = q->B, a.T = q->T, a.Hq = q->Hq, a.Hkv = q->Hkv, a.page_size = q->page_size, a.num_pages = q->num_pages;
+    while ((1 << a.page_log) < q->page_size) ++a.page_log;
+    a.window = q->window, a.sinks = q->sinks, a.splits = plan.splits, a.max_units = plan.max_units;
+    a.qk_scale_factor = q->qk_scale_factor;
+    // the largest power of two that keeps |q| * scale below 2^15 (|q| <= qk_scale_factor * sqrt(128) after RMSNorm)
+    float qs = 1.0f;
+    const float qmax = fabsf(q->qk_scale_factor) * 11.3137085f;
+    while (qs * 2.0f * qmax <= 32768.0f && qs < 65536.0f) qs *= 2.0f;
+    while (qs * qmax > 32768.0f && qs > 1.0f / 65536.0f) qs *= 0.5f;
+    a.q_scale = qs, a.s_scale = q->sm_scale * 1.4426950408889634f / qs;
+    a.q16 = reinterpret_cast<__half*>(ws + plan.q16), a.units = reinterpret_cast<int*>(ws + plan.units);
+    a.part_ml = reinterpret_cast<float*>(ws + plan.ml), a.part_o = reinterpret_cast<float*>(ws + plan.o);
+    a.status = status;
+
+    CUtensorMap tm_q, tm_k, tm_v;
+    {
+        const uint64_t dims[3] = {128, static_cast<uint64_t>(q->Hq), static_cast<uint64_t>(q->T)};
+        const uint64_t strides[2] = {256, static_cast<uint64_t>(q->Hq) * 256};
+        const uint32_t box[3] = {64, 8, kTok};
+        rc = make_tmap(&tm_q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.q16, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc != 0) return rc;
+    }
+    {
+        const uint64_t dims[4] = {128, static_cast<uint64_t>(q->Hkv), static_cast<uint64_t>(q->page_size), static_cast<uint64_t>(q->num_pages)};
+        const uint64_t strides[3] = {128, static_cast<uint64_t>(q->Hkv) * 128, static_cast<uint64_t>(q->Hkv) * 128 * q->page_size};
+        const uint32_t box[4] = {128, 1, static_cast<uint32_t>(q->page_size), 1};
+        rc = make_tmap(&tm_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, q->k_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+        if (rc == 0) rc = make_tmap(&tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, q->v_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+        if (rc != 0) return rc;
+    }
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MSK_ERR_CUDA;
+    static bool configured[64] = {};  // per device, like the attribute itself
+    if (!configured[dev]) {
+        if (cudaFuncSetAttribute(prompt_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return MSK_ERR_CUDA;
+        configured[dev] = true;
+    }
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = &attr;
+    cfg.gridDim = dim3(q->T + 1), cfg.blockDim = dim3(256), cfg.numAttrs = q->pdl ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, prompt_prep_kernel, a) != cudaSuccess) return MSK_ERR_CUDA;
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = kSmem, cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, prompt_attn_kernel, tm_q, tm_k, tm_v, a) != cudaSuccess) return MSK_ERR_CUDA;
+    if (plan.splits > 1) {
+        cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(q->T) * q->Hq + 7) / 8)), cfg.blockDim = dim3(256), cfg.dynamicSmemBytes = 0;
+        if (cudaLaunchKernelEx(&cfg, prompt_combine_kernel, a) != cudaSuccess) return MSK_ERR_CUDA;
+    }
+    return 0;
+}

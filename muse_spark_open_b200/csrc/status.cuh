@@ -26,7 +26,9 @@ enum MskKernelId : int {
     MSK_K_MOE2 = 5,
     MSK_K_COMBINE = 6,
     MSK_K_GLUE = 7,
-    MSK_K_EP = 8
+    MSK_K_EP = 8,
+    MSK_K_PROMPT = 9,
+    MSK_K_PAGES = 10
 };
 
 namespace msk {
