@@ -159,6 +159,53 @@ int msk_attn_prompt(const MskPromptParams* p, int* status, void* stream);
 /* Bytes of the workspace for a call of that shape (B, T, heads, max_pages, page_size, window, sinks, splits are read). */
 int msk_attn_prompt_scratch_bytes(const MskPromptParams* p, size_t* bytes);
 
+/* ---------------------------------------------------------------- pages of a paged cache
+ * What a serving loop does with the pages that the attention entry points read through `page_table`: give requests room,
+ * branch them, take pages back, and defragment.  All state is on the device and changed in place; nothing is read back, so
+ * every call can be captured.  `refs[p]` is the number of page-table entries that name page p; a page is free when it is 0.
+ * New pages are the lowest free ones, given out in the order of the call's rows.  Calls on one pool are ordered by their
+ * stream.  A row or page index out of range, a row that one call lists twice (extend, fork), a child that is also a parent:
+ * MSK_ERR_BOUNDS in `status`, and that entry is skipped.  No free page, or more tokens than max_pages hold:
+ * MSK_ERR_CAPACITY, and the positions concerned get no page (fork: the child is left empty).
+ * The reference has no counterpart: its inputs come with a finished page table (muse_attention_decode/reference.py:168-253).
+ */
+typedef struct {
+    int32_t* page_table;  /* [rows, max_pages], -1 = none */
+    int32_t* seq_lens;    /* [rows] tokens in the cache */
+    int32_t* refs;        /* [num_pages] */
+    int rows, max_pages, num_pages, page_size; /* page_size a power of two */
+} MskPages;
+
+/* Workspace of msk_pages_extend / fork / compact for lists of n rows (any contents, 256-byte aligned; calls that may
+ * overlap on the GPU need one each). */
+int msk_pages_scratch_bytes(const MskPages* pool, int n, size_t* bytes);
+
+/* Room for new tokens: rows[j] gets pages for the positions seq_lens .. seq_lens + n_j - 1 that have none, n_j = q_len, or
+ * cu_seqlens[j + 1] - cu_seqlens[j] when cu_seqlens is given (then `tokens` is the length of cache_loc).  seq_lens stays.
+ * cache_loc (int64, or NULL): the flat cache row of each new token, -1 where there is none; entries behind the last row's
+ * tokens are left as they were. */
+int msk_pages_extend(const MskPages* pool, const int32_t* rows, int n, int q_len, const int32_t* cu_seqlens, int tokens,
+                     int64_t* cache_loc, void* scratch, size_t scratch_bytes, int* status, void* stream);
+
+/* children[j] becomes a copy of parents[j]: full pages are shared, a last page that is not full is copied into a new one
+ * (its filled part, in each of the n_caches <= 128 caches [num_pages, page_size, token_bytes]; `caches` is a host array,
+ * read during the call).  What a child's row held goes back.  A parent may have several children; token_bytes is a multiple
+ * of 16. */
+int msk_pages_fork(const MskPages* pool, const int32_t* parents, const int32_t* children, int n, void* const* caches, int n_caches,
+                   int token_bytes, void* scratch, size_t scratch_bytes, int* status, void* stream);
+
+/* The rows' pages go back and the rows become empty (a row listed twice is freed once). */
+int msk_pages_free(const MskPages* pool, const int32_t* rows, int n, int* status, void* stream);
+
+/* The pages that no later token of the rows can see go back: those that lie wholly in [sinks, seq_lens - window].  Their
+ * table entries become -1.  window 0 (everything stays visible): nothing to do. */
+int msk_pages_trim(const MskPages* pool, const int32_t* rows, int n, int window, int sinks, int* status, void* stream);
+
+/* With n pages in use, the k-th page in use from page n on moves into the k-th free page below n, in every cache, and the
+ * table follows: afterwards the pages in use are [0, n).  result (device int32[2], or NULL): n, pages moved. */
+int msk_pages_compact(const MskPages* pool, void* const* caches, int n_caches, int token_bytes, int32_t* result, void* scratch,
+                      size_t scratch_bytes, int* status, void* stream);
+
 /* ---------------------------------------------------------------- NVFP4 (w4a16) routed experts
  * Per local (token, slot) pair: h = x . W13[e]^T, inter = fp16(silu(h[:I]) * h[I:]), y = inter . W2[e]^T,
  * out[token] += topk_weight * rmsnorm(y * (1 + post_norm_w), eps); tokens without a local pair give zeros.

@@ -58,6 +58,12 @@ def lib() -> C.CDLL:
         _lib.msk_attn_decode.argtypes = [vp, vp, vp]
         _lib.msk_attn_prompt.argtypes = [vp, vp, vp]
         _lib.msk_attn_prompt_scratch_bytes.argtypes = [vp, vp]
+        _lib.msk_pages_scratch_bytes.argtypes = [vp, ci, vp]
+        _lib.msk_pages_extend.argtypes = [vp, vp, ci, ci, vp, ci, vp, vp, C.c_size_t, vp, vp]
+        _lib.msk_pages_fork.argtypes = [vp, vp, vp, ci, vp, ci, ci, vp, C.c_size_t, vp, vp]
+        _lib.msk_pages_free.argtypes = [vp, vp, ci, vp, vp]
+        _lib.msk_pages_trim.argtypes = [vp, vp, ci, ci, ci, vp, vp]
+        _lib.msk_pages_compact.argtypes = [vp, vp, ci, ci, vp, vp, C.c_size_t, vp, vp]
         _lib.msk_moe_packed_bytes.argtypes = [ci, ci, ci, vp, vp]
         _lib.msk_moe_pack.argtypes = [vp, vp, vp, vp]
         _lib.msk_moe_dequant.argtypes = [vp, vp, ci, ci, ci, ci, vp]
@@ -84,7 +90,8 @@ def lib() -> C.CDLL:
 
 # every symbol include/msk.h declares
 EXPORTS = ["msk_version", "msk_device_info", "msk_selftest_umma", "msk_proj_skinny", "msk_proj_scratch_bytes", "msk_attn_decode",
-           "msk_attn_prompt", "msk_attn_prompt_scratch_bytes",
+           "msk_attn_prompt", "msk_attn_prompt_scratch_bytes", "msk_pages_scratch_bytes", "msk_pages_extend", "msk_pages_fork",
+           "msk_pages_free", "msk_pages_trim", "msk_pages_compact",
            "msk_moe_packed_bytes", "msk_moe_pack", "msk_moe_dequant", "msk_moe_scratch_bytes", "msk_moe_forward", "msk_moe_forward_static", "msk_layer_front", "msk_layer_decode", "msk_router", "msk_residual_boundary", "msk_rmsnorm",
            "msk_ep_row_bytes", "msk_ep_pack", "msk_ep_reduce", "msk_ep_region_bytes", "msk_ep_region_alloc", "msk_ep_region_open",
            "msk_ep_region_close", "msk_ep_region_free", "msk_ep_step", "msk_selftest_flag_timeout"]
@@ -96,6 +103,19 @@ def ptr(t: torch.Tensor | None) -> int | None:
     if not t.is_cuda:
         raise MskError("the CUDA path needs CUDA tensors; there is no CPU fallback")
     return t.data_ptr()
+
+
+def here(*tensors: torch.Tensor) -> torch.device:
+    """The device of `tensors`: all on one GPU, and that the current one (calls run on its current stream)."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev:
+            raise MskError("the tensors of one call must be on one device")
+    if dev.type != "cuda":
+        raise MskError("the CUDA path needs CUDA tensors; there is no CPU fallback")
+    if dev.index != torch.cuda.current_device():
+        raise MskError(f"the tensors are on {dev}, but the current device is cuda:{torch.cuda.current_device()}: call under torch.cuda.device(...)")
+    return dev
 
 
 def stream_ptr() -> C.c_void_p:
@@ -162,6 +182,11 @@ class PromptParams(C.Structure):
         ("qk_scale_factor", C.c_float), ("sm_scale", C.c_float), ("splits", C.c_int), ("pdl", C.c_int),
         ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
     ]
+
+
+class Pages(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("refs", C.c_void_p), ("rows", C.c_int), ("max_pages", C.c_int),
+                ("num_pages", C.c_int), ("page_size", C.c_int)]
 
 
 class MoeWeights(C.Structure):

@@ -88,11 +88,13 @@ def prompt_fn(data: dict, out: torch.Tensor | None = None, splits: int = 0) -> t
     shape = (kc.shape[0], cfg["page_size"], hkv, d)
     if kc.shape != shape or vc.shape != shape or not (kc.is_contiguous() and vc.is_contiguous()):
         raise abi.MskError("k_cache / v_cache must be contiguous [num_pages, page_size, Hkv, d]")
-    t, dev = qkv.shape[0], qkv.device
+    t, dev = qkv.shape[0], abi.here(qkv, kc, vc, data["k_scale"], data["v_scale"], seq, cu, table)
     if out is None:
         out = torch.empty((t, hq * d), dtype=torch.bfloat16, device=dev)
     elif out.dtype != torch.bfloat16 or out.shape != (t, hq * d) or out.stride(1) != 1:
         raise abi.MskError("out must be bfloat16 [tokens, Hq*d] with unit column stride")
+    else:
+        abi.here(qkv, out)
     if t == 0:
         return out
     f = inv_freq(cfg["rope_theta"], d, dev)

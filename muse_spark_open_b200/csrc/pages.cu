@@ -1,0 +1,606 @@
+// The pages of a paged cache: room for new tokens (extend), branches that share their prefix (fork), pages given back
+// (free, trim) and pages in use moved to the front (compact).
+//
+// State on the device: page_table [rows, max_pages] (physical page of each logical page, -1 = none), seq_lens [rows],
+// refs [num_pages] = table entries that name a page.  A page is free when refs is 0; new pages are always the lowest free
+// ones, in the order of the calls' rows, so that results do not depend on scheduling.  No call reads anything back to the
+// host: all of them can be captured.
+//
+// Allocation and compaction need ranks over `refs` (the k-th free page): one cluster of eight CTAs counts its slices,
+// exchanges the counts, and ranks (two reads of 4 bytes per page; a single CTA would take 4 times as long at 65536 pages,
+// a grid-wide scan a second launch).  What follows -- table rows, page data -- is a second launch over all SMs, chained
+// programmatically.  Bound by latency at small sizes, by memory (page data, read once and written once) at large ones.
+#include "msk.h"
+#include "ptx.cuh"
+
+namespace msk {
+namespace {
+
+constexpr int kCluster = 8;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kCopyThreads = 256;
+constexpr int kCopyChunk = 16384;     // bytes a CTA moves at a time: 4 x 16 per thread in flight
+constexpr int kMaxCaches = 128;
+constexpr int kWhere = MSK_K_PAGES << 8;
+
+struct Caches {
+    uint8_t* p[kMaxCaches];
+    int n;
+    int token_bytes;
+};
+
+struct PlanArgs {
+    int* page_table;
+    int* seq_lens;
+    int* refs;
+    int rows, max_pages, num_pages, page_size, page_log;
+    const int* list;       // rows to extend / children
+    const int* parents;    // fork
+    int n;
+    int q_len;             // extend: tokens per row, or
+    const int* cu;         // ... cu[n + 1]
+    int tokens;            // entries of cache_loc
+    long long* cache_loc;
+    // workspace
+    int* counts;           // [3][kCluster] slices' counts, then [4]: results
+    int* claim;            // [rows] first list entry that names a row
+    int* is_parent;        // [rows]
+    int* need;             // [n]
+    int* offs;             // [n]
+    int* free_list;        // [num_pages]
+    int4* ops;             // [n] fork: source page, new page, tokens to copy, 1 = done / 0 = refused / 2 = no page
+    int* src;              // [num_pages] compact: moved pages ...
+    int* dst;              // ... and where to
+    int* remap;            // [num_pages]
+    int* result;           // compact: pages in use, pages moved; or NULL
+    int* status;
+};
+
+// (exclusive prefix of v over the CTA's threads, total) -- kPlanThreads threads.
+__device__ __forceinline__ int block_scan(int v, int* total) {
+    __shared__ int part[kPlanWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+    }
+    __syncthreads();  // the previous call's readers are done
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    const int w = part[lane];
+    int winc = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, winc, o);
+        if (lane >= o) winc += u;
+    }
+    *total = __shfl_sync(0xffffffffu, winc, 31);
+    const int before = __shfl_sync(0xffffffffu, winc - w, warp);
+    return before + inc - v;
+}
+
+__device__ __forceinline__ void cluster_exchange() {  // everything written so far, global memory included, is visible after it
+    __threadfence();
+    cluster_sync_all();
+}
+
+// Walks the pages [lo, hi) of `refs`, four per thread and step: f(first page, r[4], how many) for every thread and step
+// (the same number of steps for every thread).
+template <class F>
+__device__ __forceinline__ void walk_refs(const int* refs, int lo, int hi, F f) {
+    for (int at = lo; at < hi; at += 4 * kPlanThreads) {
+        const int i = at + 4 * static_cast<int>(threadIdx.x);
+        int r[4] = {0, 0, 0, 0};
+        const int k = min(max(hi - i, 0), 4);
+        if (k == 4 && (reinterpret_cast<uintptr_t>(refs + i) & 15) == 0) {
+            const int4 v = __ldcg(reinterpret_cast<const int4*>(refs + i));
+            r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+        } else {
+            for (int j = 0; j < k; ++j) r[j] = __ldcg(refs + i + j);
+        }
+        f(i, r, k);
+    }
+}
+
+__device__ __forceinline__ void slice_of(const PlanArgs& p, int rank, int* lo, int* hi) {  // multiples of four pages
+    const int per = ((p.num_pages + kCluster - 1) / kCluster + 3) & ~3;
+    *lo = min(rank * per, p.num_pages);
+    *hi = min(*lo + per, p.num_pages);
+}
+
+__device__ __forceinline__ int slice_total(const int* counts, int rank, int* before) {
+    int total = 0;
+    *before = 0;
+    for (int r = 0; r < kCluster; ++r) {
+        const int v = __ldcg(counts + r);
+        if (r < rank) *before += v;
+        total += v;
+    }
+    return total;
+}
+
+// The new tokens of list entry j: [first logical page, last] of row; tokens.
+__device__ __forceinline__ void span_of(const PlanArgs& p, int row, int j, int* seq, int* n_tok, int* first_loc) {
+    *seq = p.seq_lens[row];
+    if (p.cu != nullptr) {
+        const int a = min(max(p.cu[j], 0), p.tokens), b = min(max(p.cu[j + 1], 0), p.tokens);
+        *first_loc = a, *n_tok = max(b - a, 0);
+    } else {
+        *first_loc = j * p.q_len, *n_tok = p.q_len;
+    }
+}
+
+// One cluster: gives list entries the free pages they need.  kFork: one page for a child whose parent ends inside a page.
+template <bool kFork>
+__global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1) pages_plan_kernel(PlanArgs p) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = static_cast<int>(cluster_ctarank());
+    const int gtid = rank * kPlanThreads + tid, gwarp = rank * kPlanWarps + warp;
+    constexpr int kAll = kCluster * kPlanThreads, kAllWarps = kCluster * kPlanWarps;
+    pdl_wait();
+    pdl_launch_dependents();
+    // which list entry speaks for a row: the first that names it
+    for (int r = gtid; r < p.rows; r += kAll) {
+        p.claim[r] = 0x7fffffff;
+        if (kFork) p.is_parent[r] = 0;
+    }
+    int lo, hi;
+    slice_of(p, rank, &lo, &hi);
+    int mine = 0;
+    walk_refs(p.refs, lo, hi, [&](int, const int (&r)[4], int k) {
+        for (int j = 0; j < 4; ++j) mine += j < k && r[j] == 0;
+    });
+    int slice_free;
+    block_scan(mine, &slice_free);
+    if (tid == 0) p.counts[rank] = slice_free;
+    cluster_exchange();
+    for (int j = gtid; j < p.n; j += kAll) {
+        const int row = p.list[j];
+        if (row >= 0 && row < p.rows) atomicMin(p.claim + row, j);
+        if (kFork) {
+            const int par = p.parents[j];
+            if (par >= 0 && par < p.rows) atomicExch(p.is_parent + par, 1);
+        }
+    }
+    cluster_exchange();
+    // what each entry needs: a warp per entry, a lane per page
+    for (int j = gwarp; j < p.n; j += kAllWarps) {
+        const int row = p.list[j];
+        bool ok = row >= 0 && row < p.rows && __ldcg(p.claim + row) == j;
+        int need = 0;
+        if (kFork) {
+            const int par = p.parents[j];
+            ok = ok && par >= 0 && par < p.rows && __ldcg(p.is_parent + row) == 0;
+            if (lane == 0) {
+                int4 op = make_int4(-1, -1, 0, 0);
+                if (ok) {
+                    const int seq = max(p.seq_lens[par], 0), full = seq >> p.page_log, part = seq & (p.page_size - 1);
+                    op.w = 1;
+                    if (full + (part > 0) > p.max_pages) {
+                        op.w = 0;
+                        ok = false;
+                    } else if (part > 0) {
+                        op.x = p.page_table[static_cast<size_t>(par) * p.max_pages + full];
+                        op.z = part;
+                        if (op.x >= p.num_pages || op.x < 0) op.x = -1;
+                        need = op.x >= 0;
+                    }
+                }
+                if (op.w == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 1, row, j);
+                p.ops[j] = op;
+            }
+            need = __shfl_sync(0xffffffffu, need, 0);
+        } else {
+            if (!ok && lane == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 2, row, j);
+            if (ok) {
+                int seq, n_tok, first_loc;
+                span_of(p, row, j, &seq, &n_tok, &first_loc);
+                ok = seq >= 0;
+                const int first = seq >> p.page_log;
+                const int last = n_tok > 0 ? static_cast<int>((static_cast<long long>(seq) + n_tok - 1) >> p.page_log) : first - 1;
+                if (ok && last >= p.max_pages && lane == 0) report(p.status, MSK_ERR_CAPACITY, kWhere | 3, last, p.max_pages);
+                for (int lp = first + lane; __any_sync(0xffffffffu, ok && lp <= min(last, p.max_pages - 1)); lp += 32) {
+                    const bool want = ok && lp <= min(last, p.max_pages - 1) && p.page_table[static_cast<size_t>(row) * p.max_pages + lp] < 0;
+                    need += __popc(__ballot_sync(0xffffffffu, want));
+                }
+            }
+        }
+        if (lane == 0) p.need[j] = ok ? need : (kFork ? 0 : -1);  // extend: -1 = refused
+    }
+    cluster_exchange();
+    // offsets of the entries (every CTA scans the whole list and keeps those its warps will serve), and the free list
+    int total_need = 0;
+    for (int j0 = 0; j0 < p.n; j0 += kPlanThreads) {
+        const int j = j0 + tid;
+        const int v = j < p.n ? max(__ldcg(p.need + j), 0) : 0;
+        int total;
+        const int before = block_scan(v, &total);
+        if (j < p.n && (j % kAllWarps) / kPlanWarps == rank) p.offs[j] = total_need + before;
+        total_need += total;
+    }
+    int before;
+    const int total_free = slice_total(p.counts, rank, &before);
+    if (total_need > 0 && before < total_need) {
+        int at = before;
+        walk_refs(p.refs, lo, hi, [&](int i, const int (&r)[4], int k) {
+            int c = 0;
+            for (int j = 0; j < 4; ++j) c += j < k && r[j] == 0;
+            int total;
+            int w = at + block_scan(c, &total);
+            at += total;
+            for (int j = 0; j < 4; ++j)
+                if (j < k && r[j] == 0) {
+                    if (w < total_need) p.free_list[w] = i + j;
+                    ++w;
+                }
+        });
+    }
+    if (gtid == 0 && total_need > total_free) report(p.status, MSK_ERR_CAPACITY, kWhere | 4, total_need, total_free);
+    cluster_exchange();
+    for (int j = gwarp; j < p.n; j += kAllWarps) {
+        const int need = __ldcg(p.need + j), off = __ldcg(p.offs + j);
+        if (kFork) {
+            if (lane == 0 && need > 0) {
+                const bool got = off < total_free;
+                const int page = got ? __ldcg(p.free_list + off) : -1;
+                p.ops[j].y = page;
+                if (got) p.refs[page] = 1;
+                else p.ops[j].w = 2;
+            }
+            continue;
+        }
+        const int row = p.list[j];
+        int seq = 0, n_tok = 0, first_loc = 0;
+        if (row >= 0 && row < p.rows) span_of(p, row, j, &seq, &n_tok, &first_loc);
+        else if (p.cu == nullptr) first_loc = j * p.q_len, n_tok = p.q_len;
+        else first_loc = min(max(p.cu[j], 0), p.tokens), n_tok = max(min(max(p.cu[j + 1], 0), p.tokens) - first_loc, 0);
+        int* held = need >= 0 ? p.page_table + static_cast<size_t>(row) * p.max_pages : nullptr;
+        if (need > 0) {
+            const int first = seq >> p.page_log;
+            const int last = min(static_cast<int>((static_cast<long long>(seq) + n_tok - 1) >> p.page_log), p.max_pages - 1);
+            int at = off;
+            for (int lp0 = first; lp0 <= last; lp0 += 32) {
+                const int lp = lp0 + lane;
+                const bool want = lp <= last && held[lp] < 0;
+                const uint32_t all = __ballot_sync(0xffffffffu, want);
+                const int k = at + __popc(all & ((1u << lane) - 1u));
+                if (want && k < total_free) {
+                    const int page = __ldcg(p.free_list + k);
+                    held[lp] = page;
+                    p.refs[page] = 1;
+                }
+                at += __popc(all);
+            }
+            __syncwarp();
+        }
+        if (p.cache_loc != nullptr) {
+            for (int t = lane; t < n_tok; t += 32) {
+                const long long pos = static_cast<long long>(seq) + t;
+                const int page = held != nullptr && (pos >> p.page_log) < p.max_pages ? held[pos >> p.page_log] : -1;
+                p.cache_loc[static_cast<long long>(first_loc) + t] =
+                    page >= 0 ? (static_cast<long long>(page) << p.page_log) + (pos & (p.page_size - 1)) : -1;
+            }
+        }
+    }
+}
+
+// Entries of the listed rows go back: all of them (free) or those wholly before the window and behind the sinks (trim).
+__global__ void __launch_bounds__(256) pages_drop_kernel(PlanArgs p, int blocks_per_row, int window, int sinks, int trim) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int j = blockIdx.x / blocks_per_row, part = blockIdx.x % blocks_per_row;
+    const int row = p.list[j];
+    if (row < 0 || row >= p.rows) {
+        if (part == 0 && threadIdx.x == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 5, row, p.rows);
+        return;
+    }
+    int first = 0, last = p.max_pages;
+    if (trim) {
+        // the next token, at position seq, sees what lies behind seq - window: pages that end there or earlier go
+        const long long low = static_cast<long long>(p.seq_lens[row]) - window + 1;
+        first = static_cast<int>((static_cast<long long>(sinks) + p.page_size - 1) >> p.page_log);
+        last = low > 0 ? static_cast<int>(min(low >> p.page_log, static_cast<long long>(p.max_pages))) : 0;
+    }
+    for (int lp = first + part * 256 + static_cast<int>(threadIdx.x); lp < last; lp += blocks_per_row * 256) {
+        int* e = p.page_table + static_cast<size_t>(row) * p.max_pages + lp;
+        if (*e >= 0) {
+            const int id = atomicExch(e, -1);  // a row that is listed twice gives its pages back once
+            if (id >= p.num_pages) report(p.status, MSK_ERR_BOUNDS, kWhere | 6, id, p.num_pages);
+            else if (id >= 0) atomicSub(p.refs + id, 1);
+        }
+    }
+    if (!trim && part == 0 && threadIdx.x == 0) p.seq_lens[row] = 0;
+}
+
+// `bytes` (a multiple of 16) from src to dst by one CTA, in flight kCopyChunk at a time.
+__device__ __forceinline__ void copy_chunk(uint8_t* dst, const uint8_t* src, int bytes) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int at = (u * kCopyThreads + static_cast<int>(threadIdx.x)) * 16;
+        if (at < bytes) v[u] = __ldcs(reinterpret_cast<const uint4*>(src + at));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int at = (u * kCopyThreads + static_cast<int>(threadIdx.x)) * 16;
+        if (at < bytes) __stcs(reinterpret_cast<uint4*>(dst + at), v[u]);
+    }
+}
+
+// Fork, second launch: the children's table rows, the shared pages' counts, and the data of the pages that are copied.
+// CTAs [0, row_blocks) do the rows, the others the data.
+__global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(PlanArgs p, Caches caches, int row_blocks, int blocks_per_row) {
+    pdl_wait();
+    pdl_launch_dependents();
+    if (static_cast<int>(blockIdx.x) < row_blocks) {
+        const int j = blockIdx.x / blocks_per_row, part = blockIdx.x % blocks_per_row;
+        const int4 op = __ldcg(p.ops + j);
+        if (op.w == 0) return;
+        const int child = p.list[j], par = p.parents[j];
+        const int seq = max(p.seq_lens[par], 0), full = seq >> p.page_log;
+        for (int lp = part * kCopyThreads + static_cast<int>(threadIdx.x); lp < p.max_pages; lp += blocks_per_row * kCopyThreads) {
+            int* e = p.page_table + static_cast<size_t>(child) * p.max_pages + lp;
+            const int old = *e;
+            int id = -1;
+            if (op.w == 1) id = lp < full ? p.page_table[static_cast<size_t>(par) * p.max_pages + lp] : lp == full ? op.y : -1;
+            *e = id;
+            if (id >= 0 && id < p.num_pages && lp < full) atomicAdd(p.refs + id, 1);
+            if (old >= 0 && old < p.num_pages) atomicSub(p.refs + old, 1);  // what the child's row held before
+        }
+        if (part == 0 && threadIdx.x == 0) p.seq_lens[child] = op.w == 1 ? seq : 0;
+        return;
+    }
+    const int page_bytes = p.page_size * caches.token_bytes;
+    const int chunks = (page_bytes + kCopyChunk - 1) / kCopyChunk;
+    const long long units = static_cast<long long>(p.n) * caches.n * chunks;
+    for (long long u = blockIdx.x - row_blocks; u < units; u += gridDim.x - row_blocks) {
+        const int c = static_cast<int>(u % chunks), k = static_cast<int>(u / chunks % caches.n);
+        const int4 op = __ldcg(p.ops + u / chunks / caches.n);
+        const int bytes = op.z * caches.token_bytes - c * kCopyChunk;
+        if (op.w != 1 || op.y < 0 || bytes <= 0) continue;
+        const size_t at = static_cast<size_t>(c) * kCopyChunk;
+        copy_chunk(caches.p[k] + static_cast<size_t>(op.y) * page_bytes + at, caches.p[k] + static_cast<size_t>(op.x) * page_bytes + at,
+                   min(bytes, kCopyChunk));
+    }
+}
+
+// Compact, first launch (one cluster): with n pages in use, the k-th page in use from n on goes to the k-th free page below n.
+__global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1) pages_compact_plan_kernel(PlanArgs p) {
+    const int tid = threadIdx.x;
+    const int rank = static_cast<int>(cluster_ctarank());
+    const int gtid = rank * kPlanThreads + tid;
+    constexpr int kAll = kCluster * kPlanThreads;
+    pdl_wait();
+    pdl_launch_dependents();
+    int lo, hi;
+    slice_of(p, rank, &lo, &hi);
+    int mine = 0, total, before;
+    walk_refs(p.refs, lo, hi, [&](int, const int (&r)[4], int k) {
+        for (int j = 0; j < 4; ++j) mine += j < k && r[j] > 0;
+    });
+    block_scan(mine, &total);
+    if (tid == 0) p.counts[rank] = total;
+    cluster_exchange();
+    const int live = slice_total(p.counts, rank, &before);
+    // a page below `live` that is free, or one in use from `live` on: as many of the one as of the other
+    auto kind = [&](int page, int r) { return page < live ? (r <= 0 ? 1 : 0) : (r > 0 ? 2 : 0); };
+    int holes = 0, moves = 0;
+    walk_refs(p.refs, lo, hi, [&](int i, const int (&r)[4], int k) {
+        for (int j = 0; j < 4; ++j) {
+            const int t = j < k ? kind(i + j, r[j]) : 0;
+            holes += t == 1, moves += t == 2;
+        }
+    });
+    block_scan(holes, &total);
+    if (tid == 0) p.counts[kCluster + rank] = total;
+    block_scan(moves, &total);
+    if (tid == 0) p.counts[2 * kCluster + rank] = total;
+    cluster_exchange();
+    int hole_at, move_at;
+    slice_total(p.counts + kCluster, rank, &hole_at);
+    const int all_moves = slice_total(p.counts + 2 * kCluster, rank, &move_at);
+    walk_refs(p.refs, lo, hi, [&](int i, const int (&r)[4], int k) {
+        int nh = 0, nm = 0;
+        for (int j = 0; j < 4; ++j) {
+            const int t = j < k ? kind(i + j, r[j]) : 0;
+            nh += t == 1, nm += t == 2;
+        }
+        int th, tm;
+        int wh = hole_at + block_scan(nh, &th), wm = move_at + block_scan(nm, &tm);
+        hole_at += th, move_at += tm;
+        for (int j = 0; j < 4; ++j) {
+            const int t = j < k ? kind(i + j, r[j]) : 0;
+            if (t == 1) p.dst[wh++] = i + j;
+            if (t == 2) p.src[wm++] = i + j;
+        }
+    });
+    cluster_exchange();
+    for (int k = gtid; k < all_moves; k += kAll) {
+        const int s = __ldcg(p.src + k), d = __ldcg(p.dst + k);
+        p.remap[s] = d;
+        p.refs[d] = __ldcg(p.refs + s);
+        p.refs[s] = 0;
+    }
+    if (gtid == 0) {
+        p.counts[3 * kCluster] = live, p.counts[3 * kCluster + 1] = all_moves;
+        if (p.result != nullptr) p.result[0] = live, p.result[1] = all_moves;
+    }
+}
+
+// Compact, second launch: the table's entries, then the pages' data.
+__global__ void __launch_bounds__(kCopyThreads) pages_compact_kernel(PlanArgs p, Caches caches) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int live = __ldcg(p.counts + 3 * kCluster), moves = __ldcg(p.counts + 3 * kCluster + 1);
+    if (moves == 0) return;
+    const long long entries = static_cast<long long>(p.rows) * p.max_pages;
+    for (long long i = static_cast<long long>(blockIdx.x) * kCopyThreads + threadIdx.x; i < entries; i += static_cast<long long>(gridDim.x) * kCopyThreads) {
+        const int id = p.page_table[i];
+        if (id >= live && id < p.num_pages) p.page_table[i] = __ldcg(p.remap + id);
+    }
+    const int page_bytes = p.page_size * caches.token_bytes;
+    const int chunks = (page_bytes + kCopyChunk - 1) / kCopyChunk;
+    const long long units = static_cast<long long>(moves) * caches.n * chunks;
+    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+        const int c = static_cast<int>(u % chunks), k = static_cast<int>(u / chunks % caches.n);
+        const long long i = u / chunks / caches.n;
+        const size_t at = static_cast<size_t>(c) * kCopyChunk;
+        copy_chunk(caches.p[k] + static_cast<size_t>(__ldcg(p.dst + i)) * page_bytes + at,
+                   caches.p[k] + static_cast<size_t>(__ldcg(p.src + i)) * page_bytes + at, min(page_bytes - static_cast<int>(at), kCopyChunk));
+    }
+}
+
+size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+// Workspace: counts | claim, is_parent [rows] | need, offs [n] | ops [n] | three lists of pages
+size_t layout(const MskPages* q, int n, uint8_t* ws, PlanArgs* a) {
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t* p = ws + at;
+        at += up256(bytes);
+        return p;
+    };
+    int* counts = reinterpret_cast<int*>(take((3 * kCluster + 4) * 4));
+    int* claim = reinterpret_cast<int*>(take(static_cast<size_t>(q->rows) * 4));
+    int* is_parent = reinterpret_cast<int*>(take(static_cast<size_t>(q->rows) * 4));
+    int* need = reinterpret_cast<int*>(take(static_cast<size_t>(n) * 4));
+    int* offs = reinterpret_cast<int*>(take(static_cast<size_t>(n) * 4));
+    int4* ops = reinterpret_cast<int4*>(take(static_cast<size_t>(n) * 16));
+    int* src = reinterpret_cast<int*>(take(static_cast<size_t>(q->num_pages) * 4));
+    int* dst = reinterpret_cast<int*>(take(static_cast<size_t>(q->num_pages) * 4));
+    int* remap = reinterpret_cast<int*>(take(static_cast<size_t>(q->num_pages) * 4));
+    if (a != nullptr) {
+        a->counts = counts, a->claim = claim, a->is_parent = is_parent, a->need = need, a->offs = offs, a->ops = ops;
+        a->src = src, a->dst = dst, a->remap = remap, a->free_list = src;
+    }
+    return at;
+}
+
+int fill(const MskPages* q, const int* list, int n, void* scratch, size_t bytes, bool workspace, int* status, PlanArgs* a) {
+    if (q == nullptr || !q->page_table || !q->seq_lens || !q->refs || n < 0 || (n > 0 && list == nullptr)) return MSK_ERR_INVALID;
+    if (q->rows < 1 || q->max_pages < 1 || q->num_pages < 1) return MSK_ERR_UNSUPPORTED;
+    if (q->page_size < 1 || (q->page_size & (q->page_size - 1)) != 0) return MSK_ERR_UNSUPPORTED;
+    *a = PlanArgs{};
+    a->page_table = q->page_table, a->seq_lens = q->seq_lens, a->refs = q->refs;
+    a->rows = q->rows, a->max_pages = q->max_pages, a->num_pages = q->num_pages, a->page_size = q->page_size;
+    while ((1 << a->page_log) < q->page_size) ++a->page_log;
+    a->list = list, a->n = n, a->status = status;
+    if (workspace) {
+        if (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 255) != 0) return MSK_ERR_INVALID;
+        if (layout(q, n, static_cast<uint8_t*>(scratch), a) > bytes) return MSK_ERR_INVALID;
+    }
+    return 0;
+}
+
+int fill_caches(const MskPages* q, void* const* caches, int n_caches, int token_bytes, Caches* c) {
+    if (n_caches < 0 || n_caches > kMaxCaches || (n_caches > 0 && caches == nullptr)) return MSK_ERR_INVALID;
+    if (token_bytes < 16 || token_bytes % 16 != 0 || static_cast<long long>(token_bytes) * q->page_size > (1 << 30)) return MSK_ERR_UNSUPPORTED;
+    *c = Caches{};
+    c->n = n_caches, c->token_bytes = token_bytes;
+    for (int i = 0; i < n_caches; ++i) {
+        if (caches[i] == nullptr || (reinterpret_cast<uintptr_t>(caches[i]) & 15) != 0) return MSK_ERR_INVALID;
+        c->p[i] = static_cast<uint8_t*>(caches[i]);
+    }
+    return 0;
+}
+
+template <class... Params, class... Args>
+int launch(void (*kernel)(Params...), unsigned grid, unsigned block, bool chained, void* stream, Args... args) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(block), cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = &attr, cfg.numAttrs = chained ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : MSK_ERR_CUDA;
+}
+
+// CTAs for page data: enough to fill every SM, no more than there are pieces.
+unsigned copy_ctas(long long units) {
+    const long long most = 148 * 8;
+    return static_cast<unsigned>(units < 1 ? 1 : units < most ? units : most);
+}
+
+int drop(const MskPages* q, const int* rows, int n, int window, int sinks, int trim, int* status, void* stream) {
+    PlanArgs a;
+    const int rc = fill(q, rows, n, nullptr, 0, false, status, &a);
+    if (rc != 0 || n == 0) return rc;
+    const int per_row = (q->max_pages + 1023) / 1024;
+    if (static_cast<long long>(n) * per_row > 0x7fffffffll) return MSK_ERR_UNSUPPORTED;
+    return launch(pages_drop_kernel, static_cast<unsigned>(n) * per_row, 256, false, stream, a, per_row, window, sinks, trim);
+}
+
+}  // namespace
+}  // namespace msk
+
+extern "C" int msk_pages_scratch_bytes(const MskPages* q, int n, size_t* bytes) {
+    if (q == nullptr || bytes == nullptr || n < 0 || q->rows < 1 || q->num_pages < 1) return MSK_ERR_INVALID;
+    *bytes = msk::layout(q, n, nullptr, nullptr);
+    return 0;
+}
+
+extern "C" int msk_pages_free(const MskPages* q, const int32_t* rows, int n, int* status, void* stream) {
+    return msk::drop(q, rows, n, 0, 0, 0, status, stream);
+}
+
+extern "C" int msk_pages_trim(const MskPages* q, const int32_t* rows, int n, int window, int sinks, int* status, void* stream) {
+    if (window < 0 || sinks < 0) return MSK_ERR_INVALID;
+    if (window == 0) n = 0;  // every position stays visible: nothing to give back
+    return msk::drop(q, rows, n, window, sinks, 1, status, stream);
+}
+
+extern "C" int msk_pages_extend(const MskPages* q, const int32_t* rows, int n, int q_len, const int32_t* cu_seqlens, int tokens,
+                                int64_t* cache_loc, void* scratch, size_t scratch_bytes, int* status, void* stream) {
+    using namespace msk;
+    PlanArgs a;
+    const int rc = fill(q, rows, n, scratch, scratch_bytes, n > 0, status, &a);
+    if (rc != 0) return rc;
+    if (cu_seqlens == nullptr && (q_len < 0 || static_cast<long long>(n) * q_len > 0x7fffffffll)) return MSK_ERR_INVALID;
+    if (cu_seqlens != nullptr && tokens < 0) return MSK_ERR_INVALID;
+    if (n == 0) return 0;
+    a.q_len = q_len, a.cu = cu_seqlens, a.tokens = cu_seqlens != nullptr ? tokens : n * q_len;
+    a.cache_loc = reinterpret_cast<long long*>(cache_loc);
+    return launch(pages_plan_kernel<false>, kCluster, kPlanThreads, false, stream, a);
+}
+
+extern "C" int msk_pages_fork(const MskPages* q, const int32_t* parents, const int32_t* children, int n, void* const* caches, int n_caches,
+                              int token_bytes, void* scratch, size_t scratch_bytes, int* status, void* stream) {
+    using namespace msk;
+    PlanArgs a;
+    int rc = fill(q, children, n, scratch, scratch_bytes, n > 0, status, &a);
+    if (rc != 0) return rc;
+    Caches c;
+    rc = fill_caches(q, caches, n_caches, token_bytes, &c);
+    if (rc != 0 || n == 0) return rc;
+    if (parents == nullptr) return MSK_ERR_INVALID;
+    a.parents = parents;
+    const int per_row = (q->max_pages + 4 * kCopyThreads - 1) / (4 * kCopyThreads);
+    const long long row_blocks = static_cast<long long>(n) * per_row;
+    const long long chunks = (static_cast<long long>(q->page_size) * token_bytes + kCopyChunk - 1) / kCopyChunk;
+    const unsigned data = copy_ctas(static_cast<long long>(n) * n_caches * chunks);
+    if (row_blocks + data > 0x7fffffffll) return MSK_ERR_UNSUPPORTED;
+    rc = launch(pages_plan_kernel<true>, kCluster, kPlanThreads, false, stream, a);
+    if (rc != 0) return rc;
+    return launch(pages_fork_kernel, static_cast<unsigned>(row_blocks) + data, kCopyThreads, true, stream, a, c, static_cast<int>(row_blocks), per_row);
+}
+
+extern "C" int msk_pages_compact(const MskPages* q, void* const* caches, int n_caches, int token_bytes, int32_t* result, void* scratch,
+                                 size_t scratch_bytes, int* status, void* stream) {
+    using namespace msk;
+    PlanArgs a;
+    int rc = fill(q, nullptr, 0, scratch, scratch_bytes, true, status, &a);
+    if (rc != 0) return rc;
+    Caches c;
+    rc = fill_caches(q, caches, n_caches, token_bytes, &c);
+    if (rc != 0) return rc;
+    a.result = result;
+    rc = launch(pages_compact_plan_kernel, kCluster, kPlanThreads, false, stream, a);
+    if (rc != 0) return rc;
+    const long long chunks = (static_cast<long long>(q->page_size) * token_bytes + kCopyChunk - 1) / kCopyChunk;
+    const long long table = (static_cast<long long>(q->rows) * q->max_pages + kCopyThreads - 1) / kCopyThreads;
+    const long long data = static_cast<long long>(q->num_pages / 2 + 1) * n_caches * chunks;  // at most half of the pages move
+    return launch(pages_compact_kernel, copy_ctas(data > table ? data : table), kCopyThreads, true, stream, a, c);
+}

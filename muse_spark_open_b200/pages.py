@@ -1,0 +1,126 @@
+"""Pages of a paged cache: what a serving loop does with the page table that `attention` and `layer` read.
+
+`prepare(num_pages, page_size, rows, max_pages, device) -> pool`, a dict of device tensors: page_table int32 [rows,
+max_pages] (-1 = no page), seq_lens int32 [rows] (tokens in the cache), refs int32 [num_pages] (table entries that name a
+page; 0 = free), and page_size.  A row is one request; `pool["page_table"]` and `pool["seq_lens"]` (or some of their rows)
+go into the `data` of attention.kernel_fn / prompt_fn and layer.kernel_fn as they are.  Lists of rows are int32 device
+tensors.  `caches` are the tensors whose first axis is the physical page and whose second the slot, K and V of every layer
+that uses the pool.  A step of a serving loop:
+
+    loc = pages.extend(pool, rows, q_len)                 # room for the next tokens; their cache rows
+    ... attention / layer step with pool["page_table"], pool["seq_lens"], cache_loc=loc ...
+    pool["seq_lens"][rows] += q_len                       # the tokens that stay (fewer after a rejected draft)
+    pages.trim(pool, rows, window, sinks)                 # what the window has passed goes back
+
+Everything happens on the device, in place and in stream order; nothing is read back, so all calls can be captured in a CUDA
+graph.  New pages are the lowest free ones, given out in the order of the rows: results do not depend on scheduling.
+Problems with the contents (a row out of range or listed twice, no free page) are reported in the status word
+(`abi.status_for(device).raise_if_set()`), and the entries concerned are skipped; include/msk.h says how.
+The reference has no counterpart: its inputs come with a finished table (muse_attention_decode/reference.py:168-253).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import abi
+
+
+def prepare(num_pages: int, page_size: int, rows: int, max_pages: int, device="cuda") -> dict:
+    """A pool with every page free and every row empty."""
+    if page_size < 1 or page_size & (page_size - 1) or min(num_pages, rows, max_pages) < 1:
+        raise abi.MskError("page_size must be a power of two, and num_pages, rows and max_pages at least 1")
+    mk = lambda shape, v: torch.full(shape, v, dtype=torch.int32, device=device)  # noqa: E731
+    return {"page_table": mk((rows, max_pages), -1), "seq_lens": mk((rows,), 0), "refs": mk((num_pages,), 0), "page_size": page_size}
+
+
+def _args(pool: dict, *lists: torch.Tensor):
+    table, seq, refs = pool["page_table"], pool["seq_lens"], pool["refs"]
+    if not table.dtype == seq.dtype == refs.dtype == torch.int32 or table.dim() != 2 or seq.dim() != 1 or seq.shape[0] != table.shape[0] or \
+            refs.dim() != 1 or not (table.is_contiguous() and seq.is_contiguous() and refs.is_contiguous()):
+        raise abi.MskError("page_table [rows, max_pages], seq_lens [rows] and refs [num_pages] must be contiguous int32")
+    for x in lists:
+        if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
+            raise abi.MskError("lists of rows must be contiguous int32 vectors")
+    dev = abi.here(table, seq, refs, *lists)
+    q = abi.Pages(table.data_ptr(), seq.data_ptr(), refs.data_ptr(), table.shape[0], table.shape[1], refs.shape[0], pool["page_size"])
+    return q, dev
+
+
+def _scratch(q: abi.Pages, n: int, dev):
+    b = C.c_size_t()
+    abi.check(abi.lib().msk_pages_scratch_bytes(C.byref(q), n, C.byref(b)), "msk_pages_scratch_bytes")
+    # from torch's allocator, on the current stream: calls on other streams and other captured graphs get other memory
+    return torch.empty(b.value, dtype=torch.uint8, device=dev)
+
+
+def _caches(caches, pool: dict, q: abi.Pages, dev):
+    token = None
+    for c in caches:
+        if c.dim() < 3 or c.shape[0] != q.num_pages or c.shape[1] != q.page_size or not c.is_contiguous():
+            raise abi.MskError("caches must be contiguous [num_pages, page_size, ...]")
+        if c.device != dev:
+            raise abi.MskError("the tensors of one call must be on one device")
+        size = c.stride(1) * c.element_size()
+        if token is not None and size != token:
+            raise abi.MskError("the caches of one call must have the same bytes per token")
+        token = size
+    return (C.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches]), len(caches), token or 16
+
+
+def extend(pool: dict, rows: torch.Tensor, q_len: int = 1, cu_seqlens: torch.Tensor | None = None, tokens: int = 0) -> torch.Tensor:
+    """Pages for the next `q_len` tokens of each row, or for cu_seqlens[j + 1] - cu_seqlens[j] of row j (then `tokens` rows
+    in all, padding included).  Returns cache_loc int64 [len(rows) * q_len] (or [tokens]): the flat cache row of each new
+    token, -1 where there is none.  seq_lens stays: the caller advances it when the tokens are in."""
+    q, dev = _args(pool, rows) if cu_seqlens is None else _args(pool, rows, cu_seqlens)
+    n = rows.shape[0]
+    if cu_seqlens is None:
+        loc = torch.empty(n * q_len, dtype=torch.int64, device=dev)
+    else:
+        if cu_seqlens.shape[0] != n + 1:
+            raise abi.MskError("cu_seqlens must have one entry more than rows")
+        loc = torch.full((tokens,), -1, dtype=torch.int64, device=dev)
+    ws = _scratch(q, n, dev)
+    abi.check(abi.lib().msk_pages_extend(C.byref(q), rows.data_ptr(), n, q_len, abi.ptr(cu_seqlens), tokens, loc.data_ptr(), ws.data_ptr(),
+                                         ws.numel(), abi.status_for(dev).p, abi.stream_ptr()), "msk_pages_extend")
+    return loc
+
+
+def fork(pool: dict, parents: torch.Tensor, children: torch.Tensor, caches) -> None:
+    """children[j] becomes a copy of parents[j]: full pages are shared, a last page that is not full is copied (its filled
+    part, in every cache).  What the children's rows held goes back.  A parent may have several children; a child must not
+    be listed twice nor be a parent."""
+    q, dev = _args(pool, parents, children)
+    n = children.shape[0]
+    if parents.shape[0] != n:
+        raise abi.MskError("parents and children must have the same length")
+    ptrs, count, token = _caches(caches, pool, q, dev)
+    ws = _scratch(q, n, dev)
+    abi.check(abi.lib().msk_pages_fork(C.byref(q), parents.data_ptr(), children.data_ptr(), n, ptrs, count, token, ws.data_ptr(), ws.numel(),
+                                       abi.status_for(dev).p, abi.stream_ptr()), "msk_pages_fork")
+
+
+def free(pool: dict, rows: torch.Tensor) -> None:
+    """The rows' pages go back, the rows become empty."""
+    q, dev = _args(pool, rows)
+    abi.check(abi.lib().msk_pages_free(C.byref(q), rows.data_ptr(), rows.shape[0], abi.status_for(dev).p, abi.stream_ptr()), "msk_pages_free")
+
+
+def trim(pool: dict, rows: torch.Tensor, window: int, sinks: int = 0) -> None:
+    """The pages that no later token of the rows sees under this window and these sinks go back (table entries become -1)."""
+    q, dev = _args(pool, rows)
+    abi.check(abi.lib().msk_pages_trim(C.byref(q), rows.data_ptr(), rows.shape[0], window, sinks, abi.status_for(dev).p, abi.stream_ptr()),
+              "msk_pages_trim")
+
+
+def compact(pool: dict, caches) -> torch.Tensor:
+    """Moves pages in use into free ones at the front, in every cache, until the n pages in use are [0, n); the table
+    follows.  Returns int32 [2] on the device: n, and how many pages moved."""
+    q, dev = _args(pool)
+    ptrs, count, token = _caches(caches, pool, q, dev)
+    ws = _scratch(q, 0, dev)
+    result = torch.empty(2, dtype=torch.int32, device=dev)
+    abi.check(abi.lib().msk_pages_compact(C.byref(q), ptrs, count, token, result.data_ptr(), ws.data_ptr(), ws.numel(), abi.status_for(dev).p,
+                                          abi.stream_ptr()), "msk_pages_compact")
+    return result
