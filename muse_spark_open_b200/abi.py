@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -105,17 +106,32 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
-def here(*tensors: torch.Tensor) -> torch.device:
-    """The device of `tensors`: all on one GPU, and that the current one (calls run on its current stream)."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t.device != dev:
-            raise MskError("the tensors of one call must be on one device")
-    if dev.type != "cuda":
+def here(tensors) -> int:
+    """The index of the device of `tensors`: all on one GPU, and that the current one (calls run on its current stream)."""
+    index = tensors[0].get_device()
+    if index < 0:
         raise MskError("the CUDA path needs CUDA tensors; there is no CPU fallback")
-    if dev.index != torch.cuda.current_device():
-        raise MskError(f"the tensors are on {dev}, but the current device is cuda:{torch.cuda.current_device()}: call under torch.cuda.device(...)")
-    return dev
+    for t in tensors:
+        if t.get_device() != index:
+            raise MskError("the tensors of one call must be on one device")
+    if index != torch._C._cuda_getDevice():
+        raise MskError(f"the tensors are on cuda:{index}, not on the current device: call under torch.cuda.device({index})")
+    return index
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of device `index` as a cudaStream_t (torch.cuda.current_stream builds an object on every call,
+    more host time than a small kernel takes on the GPU)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def packer(params) -> struct.Struct:
+    """A ctypes parameter struct as a `struct.Struct`: one pack() of all fields in order costs a tenth of assigning them one
+    by one, and the bytes are passed where the C function takes the struct's address."""
+    code = {C.c_void_p: "P", C.c_int: "i", C.c_float: "f", C.c_size_t: "N"}
+    fmt = struct.Struct("@" + "".join(code[t] for _, t in params._fields_) + "0P")
+    assert fmt.size == C.sizeof(params)
+    return fmt
 
 
 def stream_ptr() -> C.c_void_p:
@@ -132,6 +148,7 @@ class Status:
 
     def __init__(self, device):
         self.t = torch.zeros(4, dtype=torch.int32, device=device)
+        self.address = self.t.data_ptr()
 
     @property
     def p(self) -> C.c_void_p:
@@ -148,6 +165,11 @@ class Status:
 
 
 _status: dict = {}
+
+
+def status_ptr(index: int) -> int:
+    """The address of device `index`'s status word."""
+    return (_status.get(index) or status_for(torch.device("cuda", index))).address
 
 
 def status_for(device) -> Status:

@@ -28,40 +28,52 @@ def inv_freq(theta: float, d: int, device) -> torch.Tensor | None:
     return _inv_freq[key]
 
 
+_attn_args, _prompt_args = abi.packer(abi.AttnParams), abi.packer(abi.PromptParams)
+
+
+def _run_step(qkv: int, ld_qkv: int, out: int, ld_out: int, data: dict, cfg: dict, index: int, chunks: int, stages: int, issuers: int, pdl: bool,
+              row_groups: int) -> None:
+    kc, d = data["k_cache"], cfg["head_dim"]
+    theta = cfg["rope_theta"]
+    freq = (_inv_freq.get((float(theta), d, index)) if theta else None)
+    if theta and freq is None:
+        freq = inv_freq(theta, d, kc.device)
+    table = data["page_table"]
+    args = _attn_args.pack(
+        qkv, ld_qkv, out, ld_out, abi.ptr(kc), abi.ptr(data["v_cache"]), abi.ptr(data["k_scale"]), abi.ptr(data["v_scale"]), abi.ptr(data["seq_lens"]),
+        abi.ptr(table), table.shape[1], abi.ptr(data["cache_loc"]), freq.data_ptr() if freq is not None else 0, cfg["batch"], cfg["q_len"],
+        cfg["num_q_heads"], cfg["num_kv_heads"], d, cfg["page_size"], kc.shape[0], cfg["window"], cfg["qk_scale_factor"], cfg["sm_scale"], chunks,
+        stages, issuers, int(pdl), row_groups, cfg.get("sinks", 0))
+    rc = abi.lib().msk_attn_decode(args, abi.status_ptr(index), abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_attn_decode")
+
+
 def launch(qkv2d: torch.Tensor, out2d: torch.Tensor, data: dict, cfg: dict, chunks: int = 0, stages: int = 0, issuers: int = 0,
            pdl: bool = False, row_groups: int = 0) -> None:
     """qkv2d bf16 [B*L, >= (2Hq+2Hkv)*d] (row stride free), out2d bf16 [B*L, Hq*d]."""
-    p = abi.AttnParams()
-    p.qkv, p.ld_qkv, p.out, p.ld_out = abi.ptr(qkv2d), qkv2d.stride(0), abi.ptr(out2d), out2d.stride(0)
-    kc, vc = data["k_cache"], data["v_cache"]
-    p.k_cache, p.v_cache = abi.ptr(kc), abi.ptr(vc)
-    p.k_scale, p.v_scale = abi.ptr(data["k_scale"]), abi.ptr(data["v_scale"])
-    p.seq_lens, p.page_table = abi.ptr(data["seq_lens"]), abi.ptr(data["page_table"])
-    p.max_pages = data["page_table"].shape[1]
-    p.cache_loc = abi.ptr(data["cache_loc"])
-    f = inv_freq(cfg["rope_theta"], cfg["head_dim"], qkv2d.device)
-    p.inv_freq = abi.ptr(f) if f is not None else None
-    p.B, p.L, p.Hq, p.Hkv, p.d = cfg["batch"], cfg["q_len"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"]
-    p.page_size, p.num_pages, p.window = cfg["page_size"], kc.shape[0], cfg["window"]
-    p.sinks = cfg.get("sinks", 0)
-    p.qk_scale_factor, p.sm_scale = cfg["qk_scale_factor"], cfg["sm_scale"]
-    p.chunks, p.stages, p.issuers, p.pdl, p.row_groups = chunks, stages, issuers, int(pdl), row_groups
-    st = abi.status_for(qkv2d.device)
-    abi.check(abi.lib().msk_attn_decode(C.byref(p), st.p, abi.stream_ptr()), "msk_attn_decode")
+    _run_step(abi.ptr(qkv2d), qkv2d.stride(0), abi.ptr(out2d), out2d.stride(0), data, cfg, qkv2d.get_device(), chunks, stages, issuers, pdl, row_groups)
 
 
 def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
     cfg = data["config"]
-    b, l, hq, d = cfg["batch"], cfg["q_len"], cfg["num_q_heads"], cfg["head_dim"]
+    b, l, wide = cfg["batch"], cfg["q_len"], cfg["num_q_heads"] * cfg["head_dim"]
     qkv = data["qkv"]
     if qkv.dtype != torch.bfloat16 or data["k_cache"].dtype != torch.float8_e4m3fn:
         raise abi.MskError("qkv must be bfloat16 and the cache float8_e4m3fn")
     if data["seq_lens"].dtype != torch.int32 or data["page_table"].dtype != torch.int32 or \
             data["cache_loc"].dtype != torch.int64:
         raise abi.MskError("seq_lens / page_table must be int32 and cache_loc int64")
-    out = torch.empty((b, l, hq * d), dtype=torch.bfloat16, device=qkv.device)
-    launch(qkv.view(b * l, -1), out.view(b * l, hq * d), data, cfg, chunks, stages)
+    if qkv.is_contiguous() and b * l > 0 and qkv.numel() % (b * l) == 0:
+        ld = qkv.numel() // (b * l)
+    else:
+        ld = qkv.view(b * l, -1).stride(0)
+    out = torch.empty((b, l, wide), dtype=torch.bfloat16, device=qkv.device)
+    _run_step(abi.ptr(qkv), ld, out.data_ptr(), wide, data, cfg, qkv.get_device(), chunks, stages, 0, False, 0)
     return out
+
+
+_prompt_bytes: dict = {}
 
 
 def prompt_fn(data: dict, out: torch.Tensor | None = None, splits: int = 0) -> torch.Tensor:
@@ -74,37 +86,53 @@ def prompt_fn(data: dict, out: torch.Tensor | None = None, splits: int = 0) -> t
     stream, so calls on several streams or in several captured graphs do not share it.
     """
     cfg, qkv, kc, vc = data["config"], data["qkv"], data["k_cache"], data["v_cache"]
-    table, seq, cu = data["page_table"], data["seq_lens"], data["cu_seqlens_q"]
-    b, hq, hkv, d = cfg["batch"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"]
+    table, seq, cu, ks, vs = data["page_table"], data["seq_lens"], data["cu_seqlens_q"], data["k_scale"], data["v_scale"]
+    b, hq, hkv, d, page = cfg["batch"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"], cfg["page_size"]
     if qkv.dtype != torch.bfloat16 or kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
         raise abi.MskError("qkv must be bfloat16 and the cache float8_e4m3fn")
-    if qkv.dim() != 2 or qkv.shape[1] < (2 * hq + 2 * hkv) * d or qkv.stride(1) != 1:
+    t, wide = qkv.shape if qkv.dim() == 2 else (0, 0)
+    if wide < (2 * hq + 2 * hkv) * d or qkv.stride(1) != 1:
         raise abi.MskError("qkv must be [tokens, (2Hq+2Hkv)*d] with unit column stride")
     if seq.dtype != torch.int32 or table.dtype != torch.int32 or cu.dtype != torch.int32:
         raise abi.MskError("seq_lens / page_table / cu_seqlens_q must be int32")
     if seq.numel() != b or table.dim() != 2 or table.shape[0] != b or cu.numel() != b + 1 or \
             not (seq.is_contiguous() and table.is_contiguous() and cu.is_contiguous()):
         raise abi.MskError("seq_lens [B], page_table [B, max_pages] and cu_seqlens_q [B + 1] must be contiguous")
-    shape = (kc.shape[0], cfg["page_size"], hkv, d)
+    shape = (kc.shape[0], page, hkv, d)
     if kc.shape != shape or vc.shape != shape or not (kc.is_contiguous() and vc.is_contiguous()):
         raise abi.MskError("k_cache / v_cache must be contiguous [num_pages, page_size, Hkv, d]")
-    t, dev = qkv.shape[0], abi.here(qkv, kc, vc, data["k_scale"], data["v_scale"], seq, cu, table)
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise abi.MskError("k_scale / v_scale must be float32")
+    index = abi.here((qkv, kc, vc, ks, vs, seq, cu, table))
+    dev = qkv.device
     if out is None:
         out = torch.empty((t, hq * d), dtype=torch.bfloat16, device=dev)
     elif out.dtype != torch.bfloat16 or out.shape != (t, hq * d) or out.stride(1) != 1:
         raise abi.MskError("out must be bfloat16 [tokens, Hq*d] with unit column stride")
     else:
-        abi.here(qkv, out)
+        abi.here((qkv, out))
     if t == 0:
         return out
-    f = inv_freq(cfg["rope_theta"], d, dev)
-    p = abi.PromptParams(
-        abi.ptr(qkv), qkv.stride(0), abi.ptr(out), out.stride(0), abi.ptr(kc), abi.ptr(vc), abi.ptr(data["k_scale"]), abi.ptr(data["v_scale"]),
-        abi.ptr(seq), abi.ptr(cu), abi.ptr(table), table.shape[1], abi.ptr(f), b, t, hq, hkv, d, cfg["page_size"], kc.shape[0],
-        cfg["window"], cfg.get("sinks", 0), cfg["qk_scale_factor"], cfg["sm_scale"], splits, 0, None, 0)
-    lib, n = abi.lib(), C.c_size_t()
-    abi.check(lib.msk_attn_prompt_scratch_bytes(C.byref(p), C.byref(n)), "msk_attn_prompt_scratch_bytes")
-    scratch = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    p.scratch, p.scratch_bytes = scratch.data_ptr(), n.value
-    abi.check(lib.msk_attn_prompt(C.byref(p), abi.status_for(dev).p, abi.stream_ptr()), "msk_attn_prompt")
+    theta, window, sinks, max_pages = cfg["rope_theta"], cfg["window"], cfg.get("sinks", 0), table.shape[1]
+    freq = inv_freq(theta, d, dev) if theta else None
+    lib = abi.lib()
+    # the workspace's size is a function of sizes alone
+    key = (b, t, hq, hkv, d, page, kc.shape[0], window, sinks, max_pages, splits)
+    nbytes = _prompt_bytes.get(key)
+    if nbytes is None:
+        n = C.c_size_t()
+        p = abi.PromptParams(B=b, T=t, Hq=hq, Hkv=hkv, d=d, page_size=page, num_pages=kc.shape[0], window=window, sinks=sinks, max_pages=max_pages,
+                             splits=splits)
+        abi.check(lib.msk_attn_prompt_scratch_bytes(C.byref(p), C.byref(n)), "msk_attn_prompt_scratch_bytes")
+        if len(_prompt_bytes) > 4096:
+            _prompt_bytes.clear()
+        nbytes = _prompt_bytes[key] = n.value
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    args = _prompt_args.pack(
+        qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), seq.data_ptr(),
+        cu.data_ptr(), table.data_ptr(), max_pages, freq.data_ptr() if freq is not None else 0, b, t, hq, hkv, d, page, kc.shape[0], window, sinks,
+        cfg["qk_scale_factor"], cfg["sm_scale"], splits, 0, scratch.data_ptr(), nbytes)
+    rc = lib.msk_attn_prompt(args, abi.status_ptr(index), abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_attn_prompt")
     return out

@@ -21,6 +21,7 @@ The reference has no counterpart: its inputs come with a finished table (muse_at
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -35,55 +36,75 @@ def prepare(num_pages: int, page_size: int, rows: int, max_pages: int, device="c
     return {"page_table": mk((rows, max_pages), -1), "seq_lens": mk((rows,), 0), "refs": mk((num_pages,), 0), "page_size": page_size}
 
 
+_pages_args = abi.packer(abi.Pages)
+_INT = torch.int32
+_bytes: dict = {}
+
+
 def _args(pool: dict, *lists: torch.Tensor):
+    """(the packed MskPages, its shape, the device) of a pool whose tensors and lists are what the C functions expect."""
     table, seq, refs = pool["page_table"], pool["seq_lens"], pool["refs"]
-    if not table.dtype == seq.dtype == refs.dtype == torch.int32 or table.dim() != 2 or seq.dim() != 1 or seq.shape[0] != table.shape[0] or \
-            refs.dim() != 1 or not (table.is_contiguous() and seq.is_contiguous() and refs.is_contiguous()):
+    if table.dtype != _INT or seq.dtype != _INT or refs.dtype != _INT or table.dim() != 2 or seq.dim() != 1 or refs.dim() != 1 or \
+            seq.shape[0] != table.shape[0] or not (table.is_contiguous() and seq.is_contiguous() and refs.is_contiguous()):
         raise abi.MskError("page_table [rows, max_pages], seq_lens [rows] and refs [num_pages] must be contiguous int32")
     for x in lists:
-        if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
+        if x.dtype != _INT or x.dim() != 1 or not x.is_contiguous():
             raise abi.MskError("lists of rows must be contiguous int32 vectors")
-    dev = abi.here(table, seq, refs, *lists)
-    q = abi.Pages(table.data_ptr(), seq.data_ptr(), refs.data_ptr(), table.shape[0], table.shape[1], refs.shape[0], pool["page_size"])
-    return q, dev
+    index = abi.here((table, seq, refs, *lists))
+    rows, most = table.shape
+    pages = refs.shape[0]
+    return _pages_args.pack(table.data_ptr(), seq.data_ptr(), refs.data_ptr(), rows, most, pages, pool["page_size"]), (rows, pages), index
 
 
-def _scratch(q: abi.Pages, n: int, dev):
-    b = C.c_size_t()
-    abi.check(abi.lib().msk_pages_scratch_bytes(C.byref(q), n, C.byref(b)), "msk_pages_scratch_bytes")
-    # from torch's allocator, on the current stream: calls on other streams and other captured graphs get other memory
-    return torch.empty(b.value, dtype=torch.uint8, device=dev)
+def _scratch(q: bytes, shape, n: int, like: torch.Tensor):
+    # the size is a function of sizes alone; the memory comes from torch's allocator, on the current stream: calls on other
+    # streams and other captured graphs get other memory
+    key = (*shape, n)
+    size = _bytes.get(key)
+    if size is None:
+        b = C.c_size_t()
+        abi.check(abi.lib().msk_pages_scratch_bytes(q, n, C.byref(b)), "msk_pages_scratch_bytes")
+        if len(_bytes) > 4096:
+            _bytes.clear()
+        size = _bytes[key] = b.value
+    return torch.empty(size, dtype=torch.uint8, device=like.device), size
 
 
-def _caches(caches, pool: dict, q: abi.Pages, dev):
-    token = None
+def _caches(caches, pool: dict, index: int):
+    """(host array of the caches' addresses, how many, bytes per token)"""
+    pages, size, token, ptrs = pool["refs"].shape[0], pool["page_size"], 0, []
     for c in caches:
-        if c.dim() < 3 or c.shape[0] != q.num_pages or c.shape[1] != q.page_size or not c.is_contiguous():
+        shape = c.shape
+        if len(shape) < 3 or shape[0] != pages or shape[1] != size or not c.is_contiguous():
             raise abi.MskError("caches must be contiguous [num_pages, page_size, ...]")
-        if c.device != dev:
+        if c.get_device() != index:
             raise abi.MskError("the tensors of one call must be on one device")
-        size = c.stride(1) * c.element_size()
-        if token is not None and size != token:
+        bytes_ = c.stride(1) * c.element_size()
+        if token and bytes_ != token:
             raise abi.MskError("the caches of one call must have the same bytes per token")
-        token = size
-    return (C.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches]), len(caches), token or 16
+        token = bytes_
+        ptrs.append(c.data_ptr())
+    return struct.pack(f"{len(ptrs)}P", *ptrs), len(ptrs), token or 16
 
 
 def extend(pool: dict, rows: torch.Tensor, q_len: int = 1, cu_seqlens: torch.Tensor | None = None, tokens: int = 0) -> torch.Tensor:
     """Pages for the next `q_len` tokens of each row, or for cu_seqlens[j + 1] - cu_seqlens[j] of row j (then `tokens` rows
     in all, padding included).  Returns cache_loc int64 [len(rows) * q_len] (or [tokens]): the flat cache row of each new
     token, -1 where there is none.  seq_lens stays: the caller advances it when the tokens are in."""
-    q, dev = _args(pool, rows) if cu_seqlens is None else _args(pool, rows, cu_seqlens)
     n = rows.shape[0]
     if cu_seqlens is None:
-        loc = torch.empty(n * q_len, dtype=torch.int64, device=dev)
+        q, shape, index = _args(pool, rows)
+        loc, cu = torch.empty(n * q_len, dtype=torch.int64, device=rows.device), 0
     else:
+        q, shape, index = _args(pool, rows, cu_seqlens)
         if cu_seqlens.shape[0] != n + 1:
             raise abi.MskError("cu_seqlens must have one entry more than rows")
-        loc = torch.full((tokens,), -1, dtype=torch.int64, device=dev)
-    ws = _scratch(q, n, dev)
-    abi.check(abi.lib().msk_pages_extend(C.byref(q), rows.data_ptr(), n, q_len, abi.ptr(cu_seqlens), tokens, loc.data_ptr(), ws.data_ptr(),
-                                         ws.numel(), abi.status_for(dev).p, abi.stream_ptr()), "msk_pages_extend")
+        loc, cu = torch.full((tokens,), -1, dtype=torch.int64, device=rows.device), cu_seqlens.data_ptr()
+    ws, size = _scratch(q, shape, n, rows)
+    rc = abi.lib().msk_pages_extend(q, rows.data_ptr(), n, q_len, cu, tokens, loc.data_ptr(), ws.data_ptr(), size, abi.status_ptr(index),
+                                    abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_pages_extend")
     return loc
 
 
@@ -91,36 +112,43 @@ def fork(pool: dict, parents: torch.Tensor, children: torch.Tensor, caches) -> N
     """children[j] becomes a copy of parents[j]: full pages are shared, a last page that is not full is copied (its filled
     part, in every cache).  What the children's rows held goes back.  A parent may have several children; a child must not
     be listed twice nor be a parent."""
-    q, dev = _args(pool, parents, children)
+    q, shape, index = _args(pool, parents, children)
     n = children.shape[0]
     if parents.shape[0] != n:
         raise abi.MskError("parents and children must have the same length")
-    ptrs, count, token = _caches(caches, pool, q, dev)
-    ws = _scratch(q, n, dev)
-    abi.check(abi.lib().msk_pages_fork(C.byref(q), parents.data_ptr(), children.data_ptr(), n, ptrs, count, token, ws.data_ptr(), ws.numel(),
-                                       abi.status_for(dev).p, abi.stream_ptr()), "msk_pages_fork")
+    ptrs, count, token = _caches(caches, pool, index)
+    ws, size = _scratch(q, shape, n, children)
+    rc = abi.lib().msk_pages_fork(q, parents.data_ptr(), children.data_ptr(), n, ptrs, count, token, ws.data_ptr(), size, abi.status_ptr(index),
+                                  abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_pages_fork")
 
 
 def free(pool: dict, rows: torch.Tensor) -> None:
     """The rows' pages go back, the rows become empty."""
-    q, dev = _args(pool, rows)
-    abi.check(abi.lib().msk_pages_free(C.byref(q), rows.data_ptr(), rows.shape[0], abi.status_for(dev).p, abi.stream_ptr()), "msk_pages_free")
+    q, _, index = _args(pool, rows)
+    rc = abi.lib().msk_pages_free(q, rows.data_ptr(), rows.shape[0], abi.status_ptr(index), abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_pages_free")
 
 
 def trim(pool: dict, rows: torch.Tensor, window: int, sinks: int = 0) -> None:
     """The pages that no later token of the rows sees under this window and these sinks go back (table entries become -1)."""
-    q, dev = _args(pool, rows)
-    abi.check(abi.lib().msk_pages_trim(C.byref(q), rows.data_ptr(), rows.shape[0], window, sinks, abi.status_for(dev).p, abi.stream_ptr()),
-              "msk_pages_trim")
+    q, _, index = _args(pool, rows)
+    rc = abi.lib().msk_pages_trim(q, rows.data_ptr(), rows.shape[0], window, sinks, abi.status_ptr(index), abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_pages_trim")
 
 
 def compact(pool: dict, caches) -> torch.Tensor:
     """Moves pages in use into free ones at the front, in every cache, until the n pages in use are [0, n); the table
     follows.  Returns int32 [2] on the device: n, and how many pages moved."""
-    q, dev = _args(pool)
-    ptrs, count, token = _caches(caches, pool, q, dev)
-    ws = _scratch(q, 0, dev)
-    result = torch.empty(2, dtype=torch.int32, device=dev)
-    abi.check(abi.lib().msk_pages_compact(C.byref(q), ptrs, count, token, result.data_ptr(), ws.data_ptr(), ws.numel(), abi.status_for(dev).p,
-                                          abi.stream_ptr()), "msk_pages_compact")
+    q, shape, index = _args(pool)
+    ptrs, count, token = _caches(caches, pool, index)
+    refs = pool["refs"]
+    ws, size = _scratch(q, shape, 0, refs)
+    result = torch.empty(2, dtype=_INT, device=refs.device)
+    rc = abi.lib().msk_pages_compact(q, ptrs, count, token, result.data_ptr(), ws.data_ptr(), size, abi.status_ptr(index), abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_pages_compact")
     return result
