@@ -35,6 +35,7 @@ constexpr int kF16Tile = 32768;             // one K or V tile as FP16
 constexpr int kF8Tile = 16384;
 constexpr int kSmem = 2 * kQBytes + 4 * kF16Tile + 2 * kF8Tile + 1024;
 constexpr float kNegRef = -1.0e30f;
+constexpr int kPolyEvery = 4;               // of the pairs of probabilities, every how manieth goes to the FMA pipe
 constexpr float kLazy = 8.0f;               // how far (in powers of two) a row's maximum may outgrow its reference
 constexpr int kMaxUnitsHeader = 4;          // ints before the unit list: their number, padding
 
@@ -271,9 +272,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* g_v = g_k + 2 * kF16Tile;
     uint8_t* g_f8 = g_v + 2 * kF16Tile;
     auto bar = [&](int i) { return smem_u32(&bars[i]); };
-    // staging full / free (K, V); operand slots full / free; queries; scores, P per row tile; output
+    // staging full / free (K, V); operand slots full / free; queries; output; scores per row tile, halves of P per row tile
     const uint32_t st_full = bar(0), st_free = bar(2), k_full = bar(4), k_free = bar(6), v_full = bar(8), v_free = bar(10),
-                   q_full = bar(12), s_done = bar(14), p_ready = bar(16), o_done = bar(18);
+                   q_full = bar(12), o_done = bar(13), s_done = bar(14), p_ready = bar(16);
 
     if (warp == 0) {
         tmem_alloc(smem_u32(&tmem_slot), 512);
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(st_full + 8 * i, 1), mbar_init(st_free + 8 * i, 4);
             mbar_init(k_full + 8 * i, 4), mbar_init(k_free + 8 * i, 1);
             mbar_init(v_full + 8 * i, 4), mbar_init(v_free + 8 * i, 1);
-            mbar_init(s_done + 8 * i, 1), mbar_init(p_ready + 8 * i, 4);
+            mbar_init(s_done + 8 * i, 1), mbar_init(p_ready + 16 * i, 4), mbar_init(p_ready + 16 * i + 8, 4);
         }
         mbar_init(q_full, 1);
         mbar_init(o_done, 1);
@@ -356,49 +357,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float mx[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    mx[c] = __uint_as_float(x[c][0]);
+                    mx[c] = max3(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][e]));
+                    for (int e = 3; e < 31; e += 2) mx[c] = max3(mx[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+                    mx[c] = fmaxf(mx[c], __uint_as_float(x[c][31]));
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
                 // the reference moves when the maximum has outgrown it by 2^kLazy (p then stays below 2^8 in FP16)
                 const bool move = (top - m) * scale > kLazy;
-                const float m_new = move ? top : m;
-                const float alpha = move ? ex2((m - m_new) * scale) : 1.0f;
-                const bool any = __any_sync(0xffffffffu, move);
-                m = m_new;
-                const float off = -m * scale;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (__any_sync(0xffffffffu, move)) {
+                    const float m_new = move ? top : m;
+                    const float alpha = move ? ex2((m - m_new) * scale) : 1.0f;
+                    m = m_new;
+                    l *= alpha;
+                    if (i > 0) {  // the accumulator follows (its last product is done: the scores came after it)
+#pragma unroll 1
+                        for (int c = 0; c < 128; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(t_o + c, o);
+                            tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tmem_st16(t_o + c, o);
+                        }
+                    }
+                }
+                const float2 scale2 = make_float2(scale, scale), off2 = make_float2(-m * scale, -m * scale);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {  // 64 keys at a time: the first product starts under the second half
                     uint32_t w[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const int cc = c + (e >> 4), k = 2 * (e & 15);
-                        const float a = ex2(fmaf(__uint_as_float(x[cc][k]), scale, off));
-                        const float bb = ex2(fmaf(__uint_as_float(x[cc][k + 1]), scale, off));
-                        sum[(e & 1) * 2] += a;
-                        sum[(e & 1) * 2 + 1] += bb;
-                        w[e] = pack_half(a, bb);
+                        const int cc = 2 * half + (e >> 4), k = 2 * (e & 15);
+                        const float2 y = fma2(make_float2(__uint_as_float(x[cc][k]), __uint_as_float(x[cc][k + 1])), scale2, off2);
+                        const float2 v = e % kPolyEvery == kPolyEvery - 1 ? ex2_poly2(y) : make_float2(ex2(y.x), ex2(y.y));
+                        sum[e & 1] = add2(sum[e & 1], v);
+                        w[e] = pack_half(v.x, v.y);
                     }
-                    tmem_st32(t_s + 16 * c, w);
+                    tmem_st32(t_s + 32 * half, w);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready + 16 * g + 8 * half);
                 }
-                l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-                if (any && i > 0) {  // the accumulator follows the reference (its last product is done: S came after it)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(t_o + 32 * c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(t_o + 32 * c, o);
-                    }
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready + 8 * g);
+                sum[0] = add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
             }
             if (nt > 0) {
                 ok = mbar_wait(o_done, 0, p.status, where | 4) && ok;
@@ -477,58 +481,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         reg_dec<64>();
         if (warp == 12) {
-            // ================ the MMA thread
-            if (lane == 0 && nt > 0) {
+            // ================ the MMA warp: all lanes run the loop, one issues
+            if (nt > 0) {
+                const uint32_t leader = elect_one();
                 const uint32_t id_qk = umma_idesc(128, 128, 0, 0, 0, 0), id_pv = umma_idesc(128, 128, 0, 0, 0, 1);
+                const uint64_t d_q = umma_smem_desc(s_q, 16, 1024, kSwizzle128), d_k = umma_smem_desc(s_k, 16, 1024, kSwizzle128);
+                const uint64_t d_v = umma_smem_desc(s_v, 16384, 1024, kSwizzle128);
                 auto scores = [&](int g, int slot) {  // S_g = Q_g K^T
-                    const uint64_t a = umma_smem_desc(s_q + g * kQBytes, 16, 1024, kSwizzle128);
-                    const uint64_t k = umma_smem_desc(s_k + slot * kF16Tile, 16, 1024, kSwizzle128);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t o = ((e >> 2) * 16384 + (e & 3) * 32) >> 4;
-                        umma_f16_ss(tmem + g * 128, a + o, k + o, id_qk, e != 0);
+                        umma_f16_ss_if(leader, tmem + g * 128, d_q + (g * kQBytes >> 4) + o, d_k + (slot * kF16Tile >> 4) + o, id_qk, e != 0);
                     }
-                    umma_commit(s_done + 8 * g);
+                    umma_commit_if(leader, s_done + 8 * g);
                 };
-                auto output = [&](int g, int slot, bool first) {  // O_g (+)= P_g V
-                    const uint64_t v = umma_smem_desc(s_v + slot * kF16Tile, 16384, 1024, kSwizzle128);
+                auto output = [&](int g, int slot, bool first, int par) {  // O_g (+)= P_g V, each half as soon as it is there
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        umma_f16_ts(tmem + 256 + g * 128, tmem + g * 128 + 8 * e, v + ((2048 * e) >> 4), id_pv, !first || e != 0);
+                    for (int half = 0; half < 2; ++half) {
+                        if (!mbar_wait(p_ready + 16 * g + 8 * half, par, p.status, where | (10 + g))) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int e = 4 * half; e < 4 * half + 4; ++e)
+                            umma_f16_ts_if(leader, tmem + 256 + g * 128, tmem + g * 128 + 8 * e, d_v + ((slot * kF16Tile + 2048 * e) >> 4), id_pv,
+                                           !first || e != 0);
+                    }
+                    return true;
                 };
                 bool ok = mbar_wait(q_full, 0, p.status, where | 7) && mbar_wait(k_full, 0, p.status, where | 8);
                 if (ok) {
                     tc_fence_after();
                     scores(0, 0);
                     if (two) scores(1, 0);
-                    umma_commit(k_free);
+                    umma_commit_if(leader, k_free);
                 }
                 for (int i = 0; i < nt && ok; ++i) {
                     const int slot = i & 1, nslot = slot ^ 1;
-                    ok = mbar_wait(v_full + 8 * slot, (i >> 1) & 1, p.status, where | 9) && mbar_wait(p_ready, i & 1, p.status, where | 10);
-                    if (!ok) break;
-                    tc_fence_after();
-                    output(0, slot, i == 0);
                     const bool more = i + 1 < nt;
-                    if (more) {
-                        ok = mbar_wait(k_full + 8 * nslot, ((i + 1) >> 1) & 1, p.status, where | 11);
-                        if (!ok) break;
+                    ok = mbar_wait(v_full + 8 * slot, (i >> 1) & 1, p.status, where | 9) && output(0, slot, i == 0, i & 1);
+                    if (ok && more) {
+                        ok = mbar_wait(k_full + 8 * nslot, ((i + 1) >> 1) & 1, p.status, where | 12);
                         tc_fence_after();
-                        scores(0, nslot);
+                        if (ok) scores(0, nslot);
                     }
-                    if (two) {
-                        ok = mbar_wait(p_ready + 8, i & 1, p.status, where | 12);
-                        if (!ok) break;
-                        tc_fence_after();
-                        output(1, slot, i == 0);
-                    }
-                    umma_commit(v_free + 8 * slot);
+                    if (ok && two) ok = output(1, slot, i == 0, i & 1);
+                    if (!ok) break;
+                    umma_commit_if(leader, v_free + 8 * slot);
                     if (more) {
                         if (two) scores(1, nslot);
-                        umma_commit(k_free + 8 * nslot);
+                        umma_commit_if(leader, k_free + 8 * nslot);
                     }
                 }
-                umma_commit(o_done);
+                umma_commit_if(leader, o_done);
             }
             __syncwarp();
         } else if (warp == 13 && nt > 0) {
