@@ -354,15 +354,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (!(vis & (1u << e))) x[c][e] = 0xff800000u;  // -inf
                     }
                 }
-                float mx[4];
+                float mx[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    mx[c] = max3(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+                for (int c = 0; c < 8; ++c) {
+                    auto v = [&](int e) { return __uint_as_float(x[c >> 1][16 * (c & 1) + e]); };
+                    mx[c] = max3(v(0), v(1), v(2));
 #pragma unroll
-                    for (int e = 3; e < 31; e += 2) mx[c] = max3(mx[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
-                    mx[c] = fmaxf(mx[c], __uint_as_float(x[c][31]));
+                    for (int e = 3; e < 15; e += 2) mx[c] = max3(mx[c], v(e), v(e + 1));
+                    mx[c] = fmaxf(mx[c], v(15));
                 }
-                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
                 // the reference moves when the maximum has outgrown it by 2^kLazy (p then stays below 2^8 in FP16)
                 const bool move = (top - m) * scale > kLazy;
                 if (__any_sync(0xffffffffu, move)) {
@@ -447,17 +448,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint8_t* src = g_f8 + kv * kF8Tile;
                 uint8_t* dst = (kv ? g_v : g_k) + slot * kF16Tile;
                 // 8 lanes cover 64 bytes of row r and the other 64 of row r + 1: 16-byte loads and stores without conflicts
+                // (all loads before the first store: the compiler would not move a load over a store to shared memory, and
+                // a tile took 1150 clocks of load latencies instead of 400)
+                const int r0 = w * 32 + (lane >> 2), c_even = (lane & 3) + 4 * ((lane >> 2) & 1);
+                uint4 in[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    in[u] = *reinterpret_cast<const uint4*>(src + (r0 + (u >> 1) * 8) * 128 + (c_even ^ (4 * (u & 1))) * 16);
+                if (kv && (s0 + kTile - 1 > p_last || (W > 0 && s0 <= p_first - W && s0 + kTile > snk))) {
+                    // values no token sees may be anything (even NaN): zeros, so that 0 * V stays 0
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const int pos = s0 + r0 + (u >> 1) * 8;
+                        if (pos > p_last || (W > 0 && pos <= p_first - W && pos >= snk)) in[u] = make_uint4(0, 0, 0, 0);
+                    }
+                }
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
-                    const int r = w * 32 + (u >> 1) * 8 + (lane >> 2);
-                    const int c = (lane & 3) + 4 * (((lane >> 2) ^ u) & 1);
-                    uint4 in = *reinterpret_cast<const uint4*>(src + r * 128 + c * 16);
-                    if (kv) {
-                        // values no token sees may be anything (even NaN): zeros, so that 0 * V stays 0
-                        const int pos = s0 + r;
-                        if (pos > p_last || (W > 0 && pos <= p_first - W && pos >= snk)) in = make_uint4(0, 0, 0, 0);
-                    }
-                    const uint32_t q[4] = {in.x, in.y, in.z, in.w};
+                    const int r = r0 + (u >> 1) * 8, c = c_even ^ (4 * (u & 1));
+                    const uint32_t q[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
                     uint32_t o[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
