@@ -4,20 +4,24 @@
 //   prep     one CTA per token: RMSNorm, scale and RoPE of its queries (rounded to BF16, kept as FP16 in the workspace) and
 //            keys; keys and values quantised to E4M3 and written into the pages the page table names.  One more CTA lists
 //            the work units (request, first token).  Bound by memory: 18 KB per token at 32 + 4 + 4 heads.
-//   main     one CTA per (unit of 32 new tokens, KV head, split): flash attention.  The 8 query heads of a KV head and the
-//            tokens together are the rows of the product: 2 tiles of 128 rows = 16 tokens x 8 heads.
+//   main     one CTA, or a pair of CTAs on neighbouring SMs, per (unit of 32 or 64 new tokens, KV head, split): flash
+//            attention.  The 8 query heads of a KV head and the tokens together are the rows of the product: a CTA has 2
+//            tiles of 128 rows = 16 tokens x 8 heads.
 //   combine  one warp per (token, head): joins the splits' (m, l, O); used when there are fewer units than SMs.
 //
 // Main kernel, per 128-key tile (FP16 tensor-core operands: E4M3 cache values and BF16 queries are exact in FP16, and
 // FP16 probabilities are off by 2^-12, so the result carries little more than its last rounding):
-//   copying warp     TMA boxes of the K and V pages into 2 x 16 KB of E4M3 staging
-//   converting warps E4M3 -> FP16 into the swizzled operand tiles (two slots each for K and V), rows no token sees as zeros
-//   MMA thread       S = Q K^T into TMEM (128 x 128 FP32 per row tile), O += P V with P from TMEM
+//   copying warp     TMA boxes of the K and V pages into E4M3 staging
+//   converting warps E4M3 -> FP16 into the swizzled operand tiles, value rows no token sees as zeros
+//   MMA warp         S = Q K^T into TMEM (128 x 128 FP32 per row tile), O += P V with P from TMEM
 //   softmax warps    thread = row: the row's 128 scores come from TMEM in one go, no shuffles; p = 2^(s - m) goes back as
 //                    FP16 over the scores.  The running reference m moves only when a row's maximum outgrows it by 2^8,
 //                    so the accumulator in TMEM is rescaled a few times per row, not once per tile.
 // The two row tiles take turns: while one's scores are exponentiated, the tensor cores work on the other's products.
 // TMEM: S (with P over its first half) and O, 128 columns each, for two row tiles = all 512 columns.
+// Pairs (CG = 2, tcgen05 cta_group::2): a tile's products run over both SMs, 256 rows, each CTA bringing its rows and half of
+// the K and V tile.  A single CTA is bound by shared memory: per tile 128 KB of Q and K reads, 64 KB of V, 96 KB of
+// conversion and 32 KB of TMA writes take 2560 clocks at 128 bytes each, the products 2048; a pair's CTA moves 192 KB.
 #include "attn_common.cuh"
 #include "msk.h"
 #include "ptx.cuh"
@@ -28,16 +32,24 @@ namespace {
 
 constexpr int kTile = 128;                  // keys per tile
 constexpr int kTok = 16;                    // tokens per row tile
-constexpr int kUnitTok = 2 * kTok;          // tokens per unit
 constexpr int kThreads = 512;               // softmax A | softmax B | converting | MMA, copying, two idle warps
 constexpr int kQBytes = 32768;              // one row tile of queries: two swizzled halves of 64 channels
-constexpr int kF16Tile = 32768;             // one K or V tile as FP16
-constexpr int kF8Tile = 16384;
-constexpr int kSmem = 2 * kQBytes + 4 * kF16Tile + 2 * kF8Tile + 1024;
+template <int CG>
+struct Geo {
+    static constexpr int kSlots = CG == 1 ? 2 : 3;      // FP16 operand slots, K and V each
+    static constexpr int kStages = CG == 1 ? 1 : 2;     // E4M3 staging, K and V each
+    static constexpr int kF16 = 32768 / CG;             // one CTA's part of a K tile (keys) or V tile (channels) as FP16
+    static constexpr int kF8 = 16384 / CG;
+    static constexpr int kKeys = kTile / CG;            // K rows here
+    static constexpr int kChan = 128 / CG;              // V channels here
+    static constexpr int kSmem = 2 * kQBytes + 2 * kSlots * kF16 + 2 * kStages * kF8 + 1024;
+};
+static_assert(Geo<1>::kSmem <= 231000 && Geo<2>::kSmem <= 231000, "shared memory");
 constexpr float kNegRef = -1.0e30f;
 constexpr int kPolyEvery = 4;               // of the pairs of probabilities, every how manieth goes to the FMA pipe
 constexpr float kLazy = 8.0f;               // how far (in powers of two) a row's maximum may outgrow its reference
 constexpr int kMaxUnitsHeader = 4;          // ints before the unit list: their number, padding
+constexpr int kBuckets = 256;
 
 struct PromptArgs {
     const __nv_bfloat16* qkv;
@@ -54,9 +66,11 @@ struct PromptArgs {
     int max_pages;
     const float* inv_freq;
     int B, T, Hq, Hkv, page_size, page_log, num_pages, window, sinks, splits, max_units;
+    int out_wide;     // rows of out allow 32-byte stores
     float qk_scale_factor, q_scale, s_scale;  // queries are stored times q_scale (a power of two); scores times s_scale * k_scale
     __half* q16;      // [T, Hq, 128]
-    int* units;       // [kMaxUnitsHeader + 2 * max_units]
+    int* units;       // [kMaxUnitsHeader + 4 * max_units]: request, first row of qkv, tokens, first position
+    int unit;         // tokens per unit
     float* part_o;    // [splits, T * Hq, 128]
     float* part_ml;   // [splits, T * Hq, 2]
     int* status;
@@ -84,44 +98,62 @@ __device__ __forceinline__ void norm_turn(float (&x)[4], float post_scale, const
     }
 }
 
-// The unit list: for each request its groups of 32 new tokens, the last group first (it sees the most keys, so the long
-// units start early).  One CTA.
+// How many key tiles a unit's tokens see, and where they are: [0, sink_tiles) and [first, first + tiles - sink_tiles).
+__device__ __forceinline__ int key_tiles(const PromptArgs& p, int p_first, int p_last, int* first, int* sink_tiles) {
+    const int W = p.window, snk = W > 0 ? p.sinks : 0;
+    *first = (W > 0 ? max(0, p_first - W + 1) : 0) / kTile;
+    *sink_tiles = min((min(snk, p_last + 1) + kTile - 1) / kTile, *first);
+    return p_last / kTile - *first + 1 + *sink_tiles;
+}
+
+// The unit list: each request's new tokens in groups of p.unit, the units with the most key tiles first (a counting sort over
+// the number of tiles), so that the last units to start are short.  One CTA of 256 threads: a warp per request, a lane per
+// unit.  The order inside a bucket is left to the atomics; no unit's result depends on it.
 __device__ void list_units(const PromptArgs& p) {
-    __shared__ int carry_s, warp_s[8];
+    __shared__ int hist[kBuckets], n_s[256], seq_s[256], row_s[256], sum_s[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) carry_s = 0;
-    __syncthreads();
-    for (int b0 = 0; b0 < p.B; b0 += 256) {
-        const int b = b0 + tid;
-        const int n = b < p.B ? new_tokens(p, b) : 0;
-        const int tiles = (n + kUnitTok - 1) / kUnitTok;
-        int inc = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        if (lane == 31) warp_s[warp] = inc;
-        __syncthreads();
-        int before = carry_s, total = 0;
-        for (int w = 0; w < 8; ++w) {
-            if (w < warp) before += warp_s[w];
-            total += warp_s[w];
-        }
-        const int at = before + inc - tiles;
-        for (int i = 0; i < tiles; ++i) {
-            if (at + i < p.max_units) {
-                p.units[kMaxUnitsHeader + 2 * (at + i)] = b;
-                p.units[kMaxUnitsHeader + 2 * (at + i) + 1] = (tiles - 1 - i) * kUnitTok;
+    hist[tid] = 0;
+    int total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int b0 = 0; b0 < p.B; b0 += 256) {
+            __syncthreads();
+            const int b = b0 + tid;
+            if (b < p.B) n_s[tid] = new_tokens(p, b), seq_s[tid] = p.seq_lens[b], row_s[tid] = min(max(p.cu[b], 0), p.T);
+            __syncthreads();
+            for (int r = warp; r < 256 && b0 + r < p.B; r += 8) {
+                const int n = n_s[r], units = (n + p.unit - 1) / p.unit;
+                for (int i = lane; i < units; i += 32) {
+                    const int n_tok = min(n - i * p.unit, p.unit), p_first = seq_s[r] + i * p.unit;
+                    int first, sink;
+                    const int bucket = kBuckets - 1 - min(max(key_tiles(p, p_first, p_first + n_tok - 1, &first, &sink), 0), kBuckets - 1);
+                    const int at = atomicAdd(&hist[bucket], 1);
+                    if (pass == 1 && at < p.max_units)
+                        *reinterpret_cast<int4*>(p.units + kMaxUnitsHeader + 4 * at) = make_int4(b0 + r, row_s[r] + i * p.unit, n_tok, p_first);
+                }
             }
         }
         __syncthreads();
-        if (tid == 0) carry_s += total;
-        __syncthreads();
+        if (pass == 0) {  // counts -> first places
+            const int v = hist[tid];
+            int inc = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += u;
+            }
+            if (lane == 31) sum_s[warp] = inc;
+            __syncthreads();
+            int before = 0;
+            for (int w = 0; w < 8; ++w) {
+                if (w < warp) before += sum_s[w];
+                total += sum_s[w];
+            }
+            hist[tid] = before + inc - v;
+        }
     }
     if (tid == 0) {
-        if (carry_s > p.max_units) report(p.status, MSK_ERR_CAPACITY, MSK_K_PROMPT << 8 | 1, carry_s, p.max_units);
-        p.units[0] = min(carry_s, p.max_units);
+        if (total > p.max_units) report(p.status, MSK_ERR_CAPACITY, MSK_K_PROMPT << 8 | 1, total, p.max_units);
+        p.units[0] = min(total, p.max_units);
     }
 }
 
@@ -211,129 +243,97 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// The last steps for one row held by one thread: value = o * inv, RMSNorm over 128 channels, sigmoid gate, BF16.
-// `load`: the 32 values of chunk c.
-template <class Load>
-__device__ __forceinline__ void finish_row(const PromptArgs& p, Load load, float inv, bool live, size_t token, int head) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        load(c, v);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const float o = __uint_as_float(v[i]) * inv;
-            ss += o * o;
-        }
-    }
-    const float r = inv / sqrtf(ss * (1.0f / 128.0f) + 1e-5f);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint4 g[4];
-        const __nv_bfloat16* gate = p.qkv + token * p.ld_qkv + (p.Hq + 2 * p.Hkv + head) * 128 + 32 * c;
-        if (live) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) g[i] = *reinterpret_cast<const uint4*>(gate + 8 * i);
-        }
-        uint32_t v[32];
-        load(c, v);
-        if (live) {
-            __nv_bfloat16* dst = p.out + token * p.ld_out + head * 128 + 32 * c;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t gw[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float a = __uint_as_float(v[8 * i + 2 * j]) * r / (1.0f + __expf(-bf16lo(gw[j])));
-                    const float b = __uint_as_float(v[8 * i + 2 * j + 1]) * r / (1.0f + __expf(-bf16hi(gw[j])));
-                    w[j] = pack_bf16(a, b);
-                }
-                *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-    }
+// 32 bytes to one address: a full sector per lane.
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
 }
 
+template <int CG>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, PromptArgs p) {
+    using G = Geo<CG>;
+    constexpr int NS = G::kSlots, SS = G::kStages;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[20];
+    __shared__ __align__(8) uint64_t bars[4 * SS + 4 * NS + 11];
     __shared__ uint32_t tmem_slot;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int h = blockIdx.x % p.Hkv, sp = (blockIdx.x / p.Hkv) % p.splits, slot_u = blockIdx.x / (p.Hkv * p.splits);
+    const int rank = CG == 1 ? 0 : static_cast<int>(cluster_ctarank());  // which half of the pair; the even one issues the MMAs
+    const int unit_id = blockIdx.x / CG;
+    const int h = unit_id % p.Hkv, sp = (unit_id / p.Hkv) % p.splits, slot_u = unit_id / (p.Hkv * p.splits);
     const int where = MSK_K_PROMPT << 8;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t s_q = base, s_k = s_q + 2 * kQBytes, s_v = s_k + 2 * kF16Tile, s_f8 = s_v + 2 * kF16Tile;
+    const uint32_t s_q = base, s_k = s_q + 2 * kQBytes, s_v = s_k + NS * G::kF16, s_f8 = s_v + NS * G::kF16;
     uint8_t* g_k = gbase + 2 * kQBytes;
-    uint8_t* g_v = g_k + 2 * kF16Tile;
-    uint8_t* g_f8 = g_v + 2 * kF16Tile;
+    uint8_t* g_v = g_k + NS * G::kF16;
+    uint8_t* g_f8 = g_v + NS * G::kF16;
     auto bar = [&](int i) { return smem_u32(&bars[i]); };
-    // staging full / free (K, V); operand slots full / free; queries; output; scores per row tile, halves of P per row tile
-    const uint32_t st_full = bar(0), st_free = bar(2), k_full = bar(4), k_free = bar(6), v_full = bar(8), v_free = bar(10),
-                   q_full = bar(12), o_done = bar(13), s_done = bar(14), p_ready = bar(16);
+    // staging full / free, K stages then V stages; operand slots full / free, K then V; queries; output; scores per row
+    // tile; halves of P per row tile.  With a pair, "full", "queries" and "P" collect both CTAs' arrivals at the even CTA;
+    // what the MMAs signal arrives in both.
+    const uint32_t st_full = bar(0), st_free = bar(2 * SS), op_full = bar(4 * SS), op_free = bar(4 * SS + 2 * NS),
+                   q_here = bar(4 * SS + 4 * NS), q_full = q_here + 8, o_done = q_here + 16, s_done = q_here + 32, p_ready = q_here + 48;
+    auto arrive_issuer = [&](uint32_t b) {
+        if constexpr (CG == 1) mbar_arrive(b);
+        else mbar_arrive_cluster(dsmem_addr(b, 0));
+    };
 
-    if (warp == 0) {
-        tmem_alloc(smem_u32(&tmem_slot), 512);
-        tmem_relinquish();
-    }
     if (tid == 32) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(st_full + 8 * i, 1), mbar_init(st_free + 8 * i, 4);
-            mbar_init(k_full + 8 * i, 4), mbar_init(k_free + 8 * i, 1);
-            mbar_init(v_full + 8 * i, 4), mbar_init(v_free + 8 * i, 1);
-            mbar_init(s_done + 8 * i, 1), mbar_init(p_ready + 16 * i, 4), mbar_init(p_ready + 16 * i + 8, 4);
-        }
-        mbar_init(q_full, 1);
-        mbar_init(o_done, 1);
+        for (int i = 0; i < 2 * SS; ++i) mbar_init(st_full + 8 * i, 1), mbar_init(st_free + 8 * i, 4);
+        for (int i = 0; i < 2 * NS; ++i) mbar_init(op_full + 8 * i, 4 * CG), mbar_init(op_free + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(o_done + 8 * i, 1), mbar_init(s_done + 8 * i, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(p_ready + 8 * i, 4 * CG);
+        mbar_init(q_here, 1);
+        mbar_init(q_full, CG);
         fence_mbar_init();
     }
     if (tid == 64) prefetch_tmap(&tm_q), prefetch_tmap(&tm_k), prefetch_tmap(&tm_v);
+    if (warp == 0) tmem_alloc_cg<CG>(smem_u32(&tmem_slot), 512);
     pdl_wait();
     pdl_launch_dependents();
 
-    // ---------------- this CTA's unit
-    const int n_units = p.units[0];
-    const bool have = slot_u < n_units;
-    const int b = have ? p.units[kMaxUnitsHeader + 2 * slot_u] : 0;
-    const int q0 = have ? p.units[kMaxUnitsHeader + 2 * slot_u + 1] : 0;
-    const int tok0 = min(max(p.cu[b], 0), p.T) + q0;       // first row of qkv / out
-    const int n_tok = have ? min(new_tokens(p, b) - q0, kUnitTok) : 0;
-    const int p_first = p.seq_lens[b] + q0, p_last = p_first + max(n_tok, 1) - 1;
+    // ---------------- this CTA's unit: the pair's row tile g covers tokens 16 CG g .. of the unit, this CTA 16 of them
+    const int n_units = __ldcg(p.units);
+    int4 u = make_int4(0, 0, 0, 0);
+    if (slot_u < n_units) u = __ldcg(reinterpret_cast<const int4*>(p.units + kMaxUnitsHeader + 4 * slot_u));
+    const int b = u.x, tok0 = u.y, n_tok = u.z, p_first = u.w, p_last = p_first + max(n_tok, 1) - 1;
     const int W = p.window, snk = W > 0 ? p.sinks : 0;
-    const int t_first = (W > 0 ? max(0, p_first - W + 1) : 0) / kTile;
-    const int sink_tiles = min((min(snk, p_last + 1) + kTile - 1) / kTile, t_first);
+    int t_first, sink_tiles;
+    const int tiles = key_tiles(p, p_first, p_last, &t_first, &sink_tiles);
     const int gap = t_first - sink_tiles;
-    const int tiles = have ? p_last / kTile - t_first + 1 + sink_tiles : 0;
     const int per = (tiles + p.splits - 1) / p.splits;
     const int v_begin = sp * per;
-    const int nt = max(0, min(per, tiles - v_begin));
-    const bool two = n_tok > kTok;                         // the second row tile has tokens
+    const int nt = n_tok > 0 ? max(0, min(per, tiles - v_begin)) : 0;
+    const bool two = n_tok > kTok * CG;                    // the second row tile has tokens
     auto base_of = [&](int i) { return (v_begin + i + (v_begin + i >= sink_tiles ? gap : 0)) * kTile; };
+    auto tok_of = [&](int g) { return kTok * (CG * g + rank); };  // first token of row tile g here, within the unit
 
     tc_fence_before();
-    __syncthreads();
+    __syncwarp();
+    if constexpr (CG == 1) __syncthreads();
+    else cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
 
     if (warp < 8) {
         // ================ softmax: thread = row of row tile g
         reg_inc<192>();
-        const int g = warp >> 2, row = tid & 127, j = row >> 3, head = h * 8 + (row & 7);
-        const int pos = p_first + g * kTok + j;
-        const bool live = g * kTok + j < n_tok;
-        const size_t token = static_cast<size_t>(tok0) + g * kTok + j;
+        const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
+        const int g = warp >> 2, row = tid & 127, j = tok_of(g) + (row >> 3), head = h * 8 + (row & 7);
+        const int pos = p_first + j;
+        const bool live = j < n_tok;
+        const size_t token = static_cast<size_t>(tok0) + j;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
         const float scale = k_scale * p.s_scale;
-        const int g_first = p_first + g * kTok, g_last = g_first + kTok - 1;
+        const int g_first = p_first + tok_of(g), g_last = g_first + kTok - 1;
         float m = kNegRef, l = 0.0f;
         bool ok = true;
-        if (g == 0 || two) {
+        if ((g == 0 || two) && nt > 0) {
             for (int i = 0; i < nt; ++i) {
                 ok = mbar_wait(s_done + 8 * g, i & 1, p.status, where | 3) && ok;
                 tc_fence_after();
@@ -400,156 +400,221 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(p_ready + 16 * g + 8 * half);
+                    if (lane == 0) arrive_issuer(p_ready + 16 * g + 8 * half);
                 }
                 sum[0] = add2(sum[0], sum[1]);
                 l += sum[0].x + sum[0].y;
             }
-            if (nt > 0) {
-                ok = mbar_wait(o_done, 0, p.status, where | 4) && ok;
-                ok = __all_sync(0xffffffffu, ok);
-                tc_fence_after();
+            // ---- the row's end: value = o * v_scale / l, RMSNorm over 128 channels, sigmoid gate, BF16 (or the split's part)
+            uint4 gate[16];
+            if (p.splits == 1 && live) {  // asked for before the last product is done
+                const uint4* src = reinterpret_cast<const uint4*>(p.qkv + token * p.ld_qkv + (p.Hq + 2 * p.Hkv + head) * 128);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) gate[e] = __ldg(src + e);
             }
-            auto load = [&](int c, uint32_t (&v)[32]) {
-                tmem_ld32(t_o + 32 * c, v);
-                tmem_wait_ld();
-            };
+            ok = mbar_wait(o_done + 8 * g, 0, p.status, where | 4) && ok;
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
             if (p.splits == 1) {
-                if (nt > 0 && ok) finish_row(p, load, v_scale / l, live, token, head);
+                const float inv = v_scale / l;
+                float ss = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(t_o + 32 * c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float o = __uint_as_float(v[e]) * inv;
+                        ss = fmaf(o, o, ss);
+                    }
+                }
+                const float r = inv / sqrtf(ss * (1.0f / 128.0f) + 1e-5f);
+                __nv_bfloat16* dst = p.out + token * p.ld_out + head * 128;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t v[16];
+                    tmem_ld16(t_o + 16 * c, v);
+                    tmem_wait_ld();
+                    if (live && ok) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint4 q = gate[2 * c + (e >> 2)];
+                            const uint32_t gw = (e & 3) == 0 ? q.x : (e & 3) == 1 ? q.y : (e & 3) == 2 ? q.z : q.w;
+                            const float a = __fdividef(__uint_as_float(v[2 * e]) * r, 1.0f + __expf(-bf16lo(gw)));
+                            const float d = __fdividef(__uint_as_float(v[2 * e + 1]) * r, 1.0f + __expf(-bf16hi(gw)));
+                            w[e] = pack_bf16(a, d);
+                        }
+                        if (p.out_wide) {
+                            store32(dst + 16 * c, w);
+                        } else {
+                            reinterpret_cast<uint4*>(dst)[2 * c] = make_uint4(w[0], w[1], w[2], w[3]);
+                            reinterpret_cast<uint4*>(dst)[2 * c + 1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                }
             } else {
                 const size_t r = (static_cast<size_t>(sp) * p.T + token) * p.Hq + head;
-                if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(nt > 0 && ok ? m * scale : kNegRef, nt > 0 && ok ? l : 0.0f);
-                if (nt > 0) {
+                if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(ok ? m * scale : kNegRef, ok ? l : 0.0f);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        load(c, v);
-                        if (live) {
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t v[32];
+                    tmem_ld32(t_o + 32 * c, v);
+                    tmem_wait_ld();
+                    if (live) {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4)
-                                *reinterpret_cast<uint4*>(p.part_o + r * 128 + 32 * c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        for (int e = 0; e < 32; e += 8) {
+                            const uint32_t w[8] = {v[e], v[e + 1], v[e + 2], v[e + 3], v[e + 4], v[e + 5], v[e + 6], v[e + 7]};
+                            store32(p.part_o + r * 128 + 32 * c + e, w);
                         }
                     }
                 }
             }
+        } else if (p.splits > 1 && live) {  // a split without keys
+            const size_t r = (static_cast<size_t>(sp) * p.T + token) * p.Hq + head;
+            *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(kNegRef, 0.0f);
         }
     } else if (warp < 12) {
-        // ================ converting: E4M3 staging -> FP16 operand tiles
+        // ================ converting: E4M3 staging -> FP16 operand tiles (this CTA's half of the keys of K, of the channels of V)
         reg_dec<64>();
         const int w = warp - 8;
         bool ok = true;
+        int stage = 0, st_ph = 0, slot = 0, op_ph = 0;
         for (int i = 0; i < nt && ok; ++i) {
-            const int s0 = base_of(i), slot = i & 1;
+            const int s0 = base_of(i);
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
-                ok = mbar_wait(st_full + 8 * kv, i & 1, p.status, where | 5) && ok;
-                if (i >= 2) ok = mbar_wait((kv ? v_free : k_free) + 8 * slot, ((i >> 1) - 1) & 1, p.status, where | 6) && ok;
+                ok = mbar_wait(st_full + 8 * (kv * SS + stage), st_ph, p.status, where | 5) && ok;
+                if (i >= NS) ok = mbar_wait(op_free + 8 * (kv * NS + slot), op_ph ^ 1, p.status, where | 6) && ok;
                 if (!ok) break;
-                const uint8_t* src = g_f8 + kv * kF8Tile;
-                uint8_t* dst = (kv ? g_v : g_k) + slot * kF16Tile;
-                // 8 lanes cover 64 bytes of row r and the other 64 of row r + 1: 16-byte loads and stores without conflicts
-                // (all loads before the first store: the compiler would not move a load over a store to shared memory, and
-                // a tile took 1150 clocks of load latencies instead of 400)
-                const int r0 = w * 32 + (lane >> 2), c_even = (lane & 3) + 4 * ((lane >> 2) & 1);
-                uint4 in[8];
+                const uint8_t* src = g_f8 + (kv * SS + stage) * G::kF8;
+                uint8_t* dst = (kv ? g_v : g_k) + slot * G::kF16;
+                // All loads before the first store: the compiler does not move a load over a store to shared memory, and a
+                // tile took 1150 clocks of load latencies instead of 400.
+                constexpr int U = 8 / CG;
+                uint4 in[U];
+                int rr[U], cc[U];  // row of the tile and 16-byte piece of the row (V of a pair: rows of 64 bytes)
+                if (CG == 2 && kv) {
+                    // 8 lanes: two rows of 64 contiguous bytes
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    in[u] = *reinterpret_cast<const uint4*>(src + (r0 + (u >> 1) * 8) * 128 + (c_even ^ (4 * (u & 1))) * 16);
+                    for (int e = 0; e < U; ++e) {
+                        rr[e] = w * 32 + e * 8 + (lane >> 2);
+                        cc[e] = lane & 3;
+                        in[e] = *reinterpret_cast<const uint4*>(src + rr[e] * 64 + cc[e] * 16);
+                    }
+                } else {
+                    // 8 lanes: 64 bytes of row r and the other 64 of row r + 1: no conflicts in loads or stores
+                    constexpr int kRows = G::kKeys / 4;  // rows of K per warp
+                    const int rows = kv ? 32 : kRows;
+#pragma unroll
+                    for (int e = 0; e < U; ++e) {
+                        rr[e] = w * rows + (e >> 1) * 8 + (lane >> 2);
+                        cc[e] = (lane & 3) + 4 * (((lane >> 2) ^ e) & 1);
+                        in[e] = *reinterpret_cast<const uint4*>(src + rr[e] * 128 + cc[e] * 16);
+                    }
+                }
                 if (kv && (s0 + kTile - 1 > p_last || (W > 0 && s0 <= p_first - W && s0 + kTile > snk))) {
                     // values no token sees may be anything (even NaN): zeros, so that 0 * V stays 0
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const int pos = s0 + r0 + (u >> 1) * 8;
-                        if (pos > p_last || (W > 0 && pos <= p_first - W && pos >= snk)) in[u] = make_uint4(0, 0, 0, 0);
+                    for (int e = 0; e < U; ++e) {
+                        const int at = s0 + rr[e];
+                        if (at > p_last || (W > 0 && at <= p_first - W && at >= snk)) in[e] = make_uint4(0, 0, 0, 0);
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int r = r0 + (u >> 1) * 8, c = c_even ^ (4 * (u & 1));
-                    const uint32_t q[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
+                for (int e = 0; e < U; ++e) {
+                    const uint32_t q[4] = {in[e].x, in[e].y, in[e].z, in[e].w};
                     uint32_t o[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[e]), __NV_E4M3);
-                        const __half2_raw d = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[e] >> 16), __NV_E4M3);
-                        o[2 * e] = *reinterpret_cast<const uint32_t*>(&a);
-                        o[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&d);
+                    for (int k = 0; k < 4; ++k) {
+                        const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[k]), __NV_E4M3);
+                        const __half2_raw d = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[k] >> 16), __NV_E4M3);
+                        o[2 * k] = *reinterpret_cast<const uint32_t*>(&a);
+                        o[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&d);
                     }
-                    uint8_t* half = dst + (c >> 2) * 16384;
-                    *reinterpret_cast<uint4*>(half + swz128(r, (c & 3) * 32)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<uint4*>(half + swz128(r, (c & 3) * 32 + 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+                    // 64 channels per swizzled row of 128 bytes; the second 64 behind all rows of the first
+                    uint8_t* half = dst + (cc[e] >> 2) * (kv ? 16384 : G::kKeys * 128);
+                    *reinterpret_cast<uint4*>(half + swz128(rr[e], (cc[e] & 3) * 32)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4*>(half + swz128(rr[e], (cc[e] & 3) * 32 + 16)) = make_uint4(o[4], o[5], o[6], o[7]);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(st_free + 8 * kv);
-                    mbar_arrive((kv ? v_full : k_full) + 8 * slot);
+                    mbar_arrive(st_free + 8 * (kv * SS + stage));
+                    arrive_issuer(op_full + 8 * (kv * NS + slot));
                 }
             }
+            if (++stage == SS) stage = 0, st_ph ^= 1;
+            if (++slot == NS) slot = 0, op_ph ^= 1;
         }
     } else {
         reg_dec<64>();
         if (warp == 12) {
-            // ================ the MMA warp: all lanes run the loop, one issues
-            if (nt > 0) {
+            // ================ the MMA warp: all lanes run the loop, one issues (of a pair, the even CTA's)
+            if (nt > 0 && rank == 0) {
                 const uint32_t leader = elect_one();
-                const uint32_t id_qk = umma_idesc(128, 128, 0, 0, 0, 0), id_pv = umma_idesc(128, 128, 0, 0, 0, 1);
+                const uint32_t id_qk = umma_idesc(128 * CG, 128, 0, 0, 0, 0), id_pv = umma_idesc(128 * CG, 128, 0, 0, 0, 1);
                 const uint64_t d_q = umma_smem_desc(s_q, 16, 1024, kSwizzle128), d_k = umma_smem_desc(s_k, 16, 1024, kSwizzle128);
                 const uint64_t d_v = umma_smem_desc(s_v, 16384, 1024, kSwizzle128);
+                auto wait = [&](uint32_t b, int parity, int site) { return mbar_wait<0, (CG > 1)>(b, parity, p.status, where | site); };
                 auto scores = [&](int g, int slot) {  // S_g = Q_g K^T
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const uint32_t o = ((e >> 2) * 16384 + (e & 3) * 32) >> 4;
-                        umma_f16_ss_if(leader, tmem + g * 128, d_q + (g * kQBytes >> 4) + o, d_k + (slot * kF16Tile >> 4) + o, id_qk, e != 0);
+                        const uint32_t oq = ((e >> 2) * 16384 + (e & 3) * 32) >> 4, ok_ = ((e >> 2) * (G::kKeys * 128) + (e & 3) * 32) >> 4;
+                        umma_f16_ss_if<CG>(leader, tmem + g * 128, d_q + (g * kQBytes >> 4) + oq, d_k + (slot * G::kF16 >> 4) + ok_, id_qk, e != 0);
                     }
-                    umma_commit_if(leader, s_done + 8 * g);
+                    umma_commit_if<CG>(leader, s_done + 8 * g);
                 };
                 auto output = [&](int g, int slot, bool first, int par) {  // O_g (+)= P_g V, each half as soon as it is there
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        if (!mbar_wait(p_ready + 16 * g + 8 * half, par, p.status, where | (10 + g))) return false;
+                        if (!wait(p_ready + 16 * g + 8 * half, par, 10 + g)) return false;
                         tc_fence_after();
 #pragma unroll
                         for (int e = 4 * half; e < 4 * half + 4; ++e)
-                            umma_f16_ts_if(leader, tmem + 256 + g * 128, tmem + g * 128 + 8 * e, d_v + ((slot * kF16Tile + 2048 * e) >> 4), id_pv,
-                                           !first || e != 0);
+                            umma_f16_ts_if<CG>(leader, tmem + 256 + g * 128, tmem + g * 128 + 8 * e, d_v + ((slot * G::kF16 + 2048 * e) >> 4), id_pv,
+                                               !first || e != 0);
                     }
                     return true;
                 };
-                bool ok = mbar_wait(q_full, 0, p.status, where | 7) && mbar_wait(k_full, 0, p.status, where | 8);
+                bool ok = wait(q_full, 0, 7) && wait(op_full, 0, 8);
+                tc_fence_after();
                 if (ok) {
-                    tc_fence_after();
                     scores(0, 0);
                     if (two) scores(1, 0);
-                    umma_commit_if(leader, k_free);
+                    umma_commit_if<CG>(leader, op_free);
                 }
+                int slot = 0, ph = 0;
                 for (int i = 0; i < nt && ok; ++i) {
-                    const int slot = i & 1, nslot = slot ^ 1;
                     const bool more = i + 1 < nt;
-                    ok = mbar_wait(v_full + 8 * slot, (i >> 1) & 1, p.status, where | 9) && output(0, slot, i == 0, i & 1);
+                    const int nslot = slot + 1 == NS ? 0 : slot + 1, nph = slot + 1 == NS ? ph ^ 1 : ph;
+                    ok = wait(op_full + 8 * (NS + slot), ph, 9) && output(0, slot, i == 0, i & 1);
                     if (ok && more) {
-                        ok = mbar_wait(k_full + 8 * nslot, ((i + 1) >> 1) & 1, p.status, where | 12);
+                        ok = wait(op_full + 8 * nslot, nph, 12);
                         tc_fence_after();
                         if (ok) scores(0, nslot);
                     }
                     if (ok && two) ok = output(1, slot, i == 0, i & 1);
                     if (!ok) break;
-                    umma_commit_if(leader, v_free + 8 * slot);
+                    umma_commit_if<CG>(leader, op_free + 8 * (NS + slot));
                     if (more) {
                         if (two) scores(1, nslot);
-                        umma_commit_if(leader, k_free + 8 * nslot);
+                        umma_commit_if<CG>(leader, op_free + 8 * nslot);
                     }
+                    slot = nslot, ph = nph;
                 }
-                umma_commit_if(leader, o_done);
+                umma_commit_if<CG>(leader, o_done);
+                umma_commit_if<CG>(leader, o_done + 8);
             }
             __syncwarp();
         } else if (warp == 13 && nt > 0) {
             // ================ the copying warp
             if (lane == 0) {
-                mbar_expect_tx(q_full, (two ? 2 : 1) * kQBytes);
+                mbar_expect_tx(q_here, (two ? 2 : 1) * kQBytes);
                 for (int g = 0; g < (two ? 2 : 1); ++g)
                     for (int c = 0; c < 2; ++c)
-                        tma_load_3d(s_q + g * kQBytes + c * 16384, &tm_q, q_full, 64 * c, h * 8, tok0 + g * kTok);
+                        tma_load_3d(s_q + g * kQBytes + c * 16384, &tm_q, q_here, 64 * c, h * 8, tok0 + tok_of(g));
             }
             const int ppt = kTile >> p.page_log;  // pages per tile, <= 16: lane j fetches page j
             auto page_of = [&](int i) {
@@ -561,27 +626,46 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 return id;  // -1: zeros
             };
+            // of a pair, K pages: the keys [64 rank, 64 rank + 64) of the tile; a page of 128 keys is split
+            const int key0 = lane << p.page_log;
+            const bool k_mine = lane < ppt && (CG == 1 || p.page_size == kTile || (key0 >= rank * G::kKeys && key0 < (rank + 1) * G::kKeys));
+            const int k_in_page = CG == 2 && p.page_size == kTile ? rank * G::kKeys : 0;
+            const uint32_t k_at = CG == 2 ? (p.page_size == kTile ? 0 : key0 - rank * G::kKeys) * 128 : key0 * 128;
             int id = page_of(0);
             bool ok = true;
+            int stage = 0, ph = 0;
             for (int i = 0; i < nt && ok; ++i) {
                 const int next = i + 1 < nt ? page_of(i + 1) : -1;
                 for (int kv = 0; kv < 2; ++kv) {
-                    if (i > 0) ok = mbar_wait(st_free + 8 * kv, (i - 1) & 1, p.status, where | 14) && ok;
+                    const uint32_t full = st_full + 8 * (kv * SS + stage);
+                    if (i >= SS) ok = mbar_wait(st_free + 8 * (kv * SS + stage), ph ^ 1, p.status, where | 14) && ok;
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(st_full + 8 * kv, kF8Tile);
+                    if (lane == 0) mbar_expect_tx(full, G::kF8);
                     __syncwarp();
-                    if (lane < ppt)
-                        tma_load_4d(s_f8 + kv * kF8Tile + (lane << p.page_log) * 128, kv ? &tm_v : &tm_k, st_full + 8 * kv, 0, h, 0, id);
+                    const uint32_t dst = s_f8 + (kv * SS + stage) * G::kF8;
+                    if (kv == 0) {
+                        if (k_mine) tma_load_4d(dst + k_at, &tm_k, full, 0, h, k_in_page, id);
+                    } else {
+                        if (lane < ppt) tma_load_4d(dst + key0 * G::kChan, &tm_v, full, CG == 2 ? rank * G::kChan : 0, h, 0, id);
+                    }
                 }
                 id = next;
+                if (++stage == SS) stage = 0, ph ^= 1;
             }
+            __syncwarp();
+        } else if (warp == 14 && nt > 0) {
+            // ================ this CTA's queries have arrived: tell the MMA warp
+            const bool ok = mbar_wait(q_here, 0, p.status, where | 15);
+            if (lane == 0 && ok) arrive_issuer(q_full);
             __syncwarp();
         }
     }
     tc_fence_before();
-    __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, 512);
+    __syncwarp();
+    if constexpr (CG == 1) __syncthreads();
+    else cluster_sync_all();  // nothing of this CTA's memory is needed by its pair any more
+    if (warp == 0) tmem_dealloc_cg<CG>(tmem, 512);
 }
 
 // Joins the splits of one (token, head) per warp: lane = 4 channels.
@@ -622,7 +706,7 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(PromptArgs p) {
 }
 
 struct Plan {
-    int max_units, splits;
+    int max_units, splits, cg;
     size_t q16, units, ml, o, total;  // byte offsets, and the end
 };
 
@@ -630,17 +714,20 @@ int plan_prompt(const MskPromptParams* q, Plan* plan) {
     if (q->d != 128 || q->Hkv < 1 || q->Hq != 8 * q->Hkv || q->B < 1 || q->T < 1 || q->max_pages < 1) return MSK_ERR_UNSUPPORTED;
     if (q->page_size < 8 || q->page_size > 128 || (q->page_size & (q->page_size - 1)) != 0) return MSK_ERR_UNSUPPORTED;
     if (q->window < 0 || q->sinks < 0 || q->splits < 0 || q->splits > 64) return MSK_ERR_INVALID;
-    const long long units = static_cast<long long>(q->T) / kUnitTok + q->B;  // sum of ceil(n / 32) is at most this
+    // Pairs of CTAs where requests bring more than 32 tokens on average: a unit of 64 tokens then fills both.
+    plan->cg = static_cast<long long>(q->T) > 32ll * q->B ? 2 : 1;
+    const int unit = 2 * kTok * plan->cg;
+    const long long units = static_cast<long long>(q->T) / unit + q->B;  // sum of ceil(n / unit) is at most this
     plan->max_units = static_cast<int>(units < q->T ? units : q->T);
     long long tiles = (static_cast<long long>(q->max_pages) * q->page_size + kTile - 1) / kTile;
     if (q->window > 0) {
-        const long long w = static_cast<long long>(q->window + kUnitTok) / kTile + 2 + (q->sinks + kTile - 1) / kTile;
+        const long long w = (static_cast<long long>(q->window) + unit) / kTile + 2 + (static_cast<long long>(q->sinks) + kTile - 1) / kTile;
         if (w < tiles) tiles = w;
     }
     plan->splits = q->splits;
     if (q->splits == 0) {
         // fewer units than SMs: the keys are split, down to two tiles a piece
-        const long long ctas = static_cast<long long>(plan->max_units) * q->Hkv;
+        const long long ctas = static_cast<long long>(plan->max_units) * q->Hkv * plan->cg;
         long long s = 148 / ctas;
         if (s > (tiles + 1) / 2) s = (tiles + 1) / 2;
         if (s > 32) s = 32;
@@ -650,7 +737,7 @@ int plan_prompt(const MskPromptParams* q, Plan* plan) {
     const size_t rows = static_cast<size_t>(q->T) * q->Hq;
     plan->q16 = 0;
     plan->units = up(rows * 256);
-    plan->ml = plan->units + up((kMaxUnitsHeader + 2 * static_cast<size_t>(plan->max_units)) * 4);
+    plan->ml = plan->units + up((kMaxUnitsHeader + 4 * static_cast<size_t>(plan->max_units)) * 4);
     const size_t parts = plan->splits > 1 ? static_cast<size_t>(plan->splits) * rows : 0;
     plan->o = plan->ml + up(parts * 8);
     plan->total = plan->o + up(parts * 512);
@@ -683,7 +770,7 @@ extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stre
           reinterpret_cast<uintptr_t>(q->v_cache)) & 15) != 0)
         return MSK_ERR_INVALID;
     if (!(q->sm_scale > 0.0f) || !(q->sm_scale < 1e30f)) return MSK_ERR_INVALID;
-    const long long ctas = static_cast<long long>(plan.max_units) * plan.splits * q->Hkv;
+    const long long ctas = static_cast<long long>(plan.max_units) * plan.splits * q->Hkv * plan.cg;
     if (ctas > 0x7fffffffll || static_cast<long long>(q->T) * q->Hq > 0x7fffffffll) return MSK_ERR_UNSUPPORTED;
 
     uint8_t* ws = static_cast<uint8_t*>(q->scratch);
@@ -695,7 +782,8 @@ extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stre
     a.page_table = q->page_table, a.max_pages = q->max_pages, a.inv_freq = q->inv_freq;
     a.B = q->B, a.T = q->T, a.Hq = q->Hq, a.Hkv = q->Hkv, a.page_size = q->page_size, a.num_pages = q->num_pages;
     while ((1 << a.page_log) < q->page_size) ++a.page_log;
-    a.window = q->window, a.sinks = q->sinks, a.splits = plan.splits, a.max_units = plan.max_units;
+    a.window = q->window, a.sinks = q->sinks, a.splits = plan.splits, a.max_units = plan.max_units, a.unit = 2 * kTok * plan.cg;
+    a.out_wide = ((reinterpret_cast<uintptr_t>(q->out) | static_cast<uintptr_t>(q->ld_out) * 2) & 31) == 0;
     a.qk_scale_factor = q->qk_scale_factor;
     // the largest power of two that keeps |q| * scale below 2^15 (|q| <= qk_scale_factor * sqrt(128) after RMSNorm)
     float qs = 1.0f;
@@ -718,28 +806,36 @@ extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stre
     {
         const uint64_t dims[4] = {128, static_cast<uint64_t>(q->Hkv), static_cast<uint64_t>(q->page_size), static_cast<uint64_t>(q->num_pages)};
         const uint64_t strides[3] = {128, static_cast<uint64_t>(q->Hkv) * 128, static_cast<uint64_t>(q->Hkv) * 128 * q->page_size};
-        const uint32_t box[4] = {128, 1, static_cast<uint32_t>(q->page_size), 1};
-        rc = make_tmap(&tm_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, q->k_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
-        if (rc == 0) rc = make_tmap(&tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, q->v_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+        // a pair's CTA copies half of the keys of K (at most 64 rows of a page) and half of the channels of V
+        const uint32_t size = static_cast<uint32_t>(q->page_size);
+        const uint32_t box_k[4] = {128, 1, plan.cg == 2 && size == kTile ? size / 2 : size, 1}, box_v[4] = {128u / plan.cg, 1, size, 1};
+        rc = make_tmap(&tm_k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, q->k_cache, dims, strides, box_k, CU_TENSOR_MAP_SWIZZLE_NONE);
+        if (rc == 0) rc = make_tmap(&tm_v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, q->v_cache, dims, strides, box_v, CU_TENSOR_MAP_SWIZZLE_NONE);
         if (rc != 0) return rc;
     }
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MSK_ERR_CUDA;
     static bool configured[64] = {};  // per device, like the attribute itself
     if (!configured[dev]) {
-        if (cudaFuncSetAttribute(prompt_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return MSK_ERR_CUDA;
+        if (cudaFuncSetAttribute(prompt_attn_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<1>::kSmem) != cudaSuccess ||
+            cudaFuncSetAttribute(prompt_attn_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<2>::kSmem) != cudaSuccess)
+            return MSK_ERR_CUDA;
         configured[dev] = true;
     }
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = plan.cg, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cfg.attrs = &attr;
+    cfg.attrs = attr;
     cfg.gridDim = dim3(q->T + 1), cfg.blockDim = dim3(256), cfg.numAttrs = q->pdl ? 1 : 0;
     if (cudaLaunchKernelEx(&cfg, prompt_prep_kernel, a) != cudaSuccess) return MSK_ERR_CUDA;
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = kSmem, cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, prompt_attn_kernel, tm_q, tm_k, tm_v, a) != cudaSuccess) return MSK_ERR_CUDA;
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas)), cfg.blockDim = dim3(kThreads), cfg.numAttrs = 2;
+    cfg.dynamicSmemBytes = plan.cg == 2 ? Geo<2>::kSmem : Geo<1>::kSmem;
+    if (cudaLaunchKernelEx(&cfg, plan.cg == 2 ? prompt_attn_kernel<2> : prompt_attn_kernel<1>, tm_q, tm_k, tm_v, a) != cudaSuccess) return MSK_ERR_CUDA;
+    cfg.numAttrs = 1;
     if (plan.splits > 1) {
         cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(q->T) * q->Hq + 7) / 8)), cfg.blockDim = dim3(256), cfg.dynamicSmemBytes = 0;
         if (cudaLaunchKernelEx(&cfg, prompt_combine_kernel, a) != cudaSuccess) return MSK_ERR_CUDA;

@@ -54,18 +54,38 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
+    if constexpr (CLUSTER) {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    }
     return ok != 0;
+}
+// Arrive on a barrier of another CTA of the cluster (address from dsmem_addr).  What is handed over with it -- operand tiles
+// and tensor memory that the tensor cores read -- has been made visible by fence.proxy.async or tcgen05.wait::st before;
+// the arrive itself releases at CTA scope only.  (At cluster scope it waits for all of the thread's writes, about 1100
+// clocks on the path of every tile.)
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
 }
 // Named CTA barrier over `count` threads (a multiple of 32; ids 1..15, id 0 is __syncthreads): a subset of the
 // CTA's warps meets without the others.
@@ -91,14 +111,15 @@ constexpr long long kWaitSlowPathCycles = 1ll << 20;
 // SLEEP_NS > 0: the warp sleeps between polls.  A polling warp issues instructions all the time and takes
 // issue slots from the warps of its scheduler that do the arithmetic; roles that wait long (an epilogue
 // waiting for a whole tile, a producer far ahead of its consumers) should sleep.
-template <int SLEEP_NS = 0>
+// CLUSTER: arrivals may come from other CTAs of the cluster, whose writes before them the waiting thread then sees.
+template <int SLEEP_NS = 0, bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* status, int where) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait<CLUSTER>(bar, parity)) return true;
     const long long t0 = clock64();
     uint32_t spins = 0;
     for (;;) {
         if (SLEEP_NS > 0) __nanosleep(SLEEP_NS);
-        if (mbar_try_wait(bar, parity)) return true;
+        if (mbar_try_wait<CLUSTER>(bar, parity)) return true;
         if ((++spins & 1023u) == 0) {
             const long long dt = clock64() - t0;
             if (dt > kWaitSlowPathCycles) {
@@ -233,36 +254,72 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uin
 // The same with a predicate instead of a branch: the whole warp runs the issuing loop and only the lane with `leader` != 0
 // issues.  Without divergence the descriptors stay in uniform registers; issued from an `if (lane == 0)` block they are
 // moved there one by one, which made an instruction cost about 110 clocks instead of the 64 it runs for.
+// CG: CTAs that work on one tile (cta_group).  With 2, the even CTA of a pair issues for both: A and the accumulator rows are
+// split over the pair, each CTA's shared memory holds its half of B's N, and the descriptors name the same offsets in both.
+template <int CG>
 __device__ __forceinline__ void umma_f16_ss_if(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                                uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p, q;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "setp.ne.b32 q, %5, 0;\n"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
-        : "memory");
+    if constexpr (CG == 1) {
+        asm volatile(
+            "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc),
+            "r"(accumulate), "r"(leader)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc),
+            "r"(accumulate), "r"(leader)
+            : "memory");
+    }
 }
+template <int CG>
 __device__ __forceinline__ void umma_f16_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                                uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p, q;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "setp.ne.b32 q, %5, 0;\n"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-        "}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
-        : "memory");
+    if constexpr (CG == 1) {
+        asm volatile(
+            "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc),
+            "r"(accumulate), "r"(leader)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc),
+            "r"(accumulate), "r"(leader)
+            : "memory");
+    }
 }
+// Signals `bar` (with 2 CTAs: the barrier at that offset in both) when everything issued so far by this thread has completed.
+template <int CG>
 __device__ __forceinline__ void umma_commit_if(uint32_t leader, uint32_t bar) {
-    asm volatile(
-        "{\n"
-        ".reg .pred q;\n"
-        "setp.ne.b32 q, %1, 0;\n"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
-        "}\n" ::"r"(bar), "r"(leader)
-        : "memory");
+    if constexpr (CG == 1) {
+        asm volatile(
+            "{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+            "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(leader)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n}\n" ::"r"(bar),
+            "r"(leader), "h"(static_cast<unsigned short>(3))
+            : "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc_cg(uint32_t smem_result, uint32_t ncols) {
+    if constexpr (CG == 1) {
+        tmem_alloc(smem_result, ncols);
+        tmem_relinquish();
+    } else {  // one warp of each CTA of the pair
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_result), "r"(ncols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_dealloc_cg(uint32_t taddr, uint32_t ncols) {
+    if constexpr (CG == 1) tmem_dealloc(taddr, ncols);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
 // TMEM <-> registers, shape 32x32b: a warp touches the 32 lanes of its quarter (warp_id % 4),
