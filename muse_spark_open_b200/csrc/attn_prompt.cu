@@ -15,8 +15,9 @@
 //   converting warps E4M3 -> FP16 into the swizzled operand tiles, value rows no token sees as zeros
 //   MMA warp         S = Q K^T into TMEM (128 x 128 FP32 per row tile), O += P V with P from TMEM
 //   softmax warps    thread = row: the row's 128 scores come from TMEM in one go, no shuffles; p = 2^(s - m) goes back as
-//                    FP16 over the scores.  The running reference m moves only when a row's maximum outgrows it by 2^8,
-//                    so the accumulator in TMEM is rescaled a few times per row, not once per tile.
+//                    FP16 over the scores.  The running reference m is set ahead of the maximum and moves only when a score
+//                    outgrows what FP16 holds, so the accumulator in TMEM is rescaled once or twice per row, not per tile
+//                    (800 clocks each time, in whichever warp has such a row).
 // The two row tiles take turns: while one's scores are exponentiated, the tensor cores work on the other's products.
 // TMEM: S (with P over its first half) and O, 128 columns each, for two row tiles = all 512 columns.
 // Pairs (CG = 2, tcgen05 cta_group::2): a tile's products run over both SMs, 256 rows, each CTA bringing its rows and half of
@@ -47,7 +48,8 @@ struct Geo {
 static_assert(Geo<1>::kSmem <= 231000 && Geo<2>::kSmem <= 231000, "shared memory");
 constexpr float kNegRef = -1.0e30f;
 constexpr int kPolyEvery = 4;               // of the pairs of probabilities, every how manieth goes to the FMA pipe
-constexpr float kLazy = 8.0f;               // how far (in powers of two) a row's maximum may outgrow its reference
+constexpr float kLazy = 15.0f;              // how far (in powers of two) a score may lie above its row's reference
+constexpr float kAhead = 4.0f;              // how far a new reference lies above the row's maximum
 constexpr int kMaxUnitsHeader = 4;          // ints before the unit list: their number, padding
 constexpr int kBuckets = 256;
 
@@ -364,11 +366,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mx[c] = fmaxf(mx[c], v(15));
                 }
                 const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
-                // the reference moves when the maximum has outgrown it by 2^kLazy (p then stays below 2^8 in FP16)
-                const bool move = (top - m) * scale > kLazy;
+                // A new reference lies 2^kAhead above the row's maximum and serves until a score lies 2^kLazy above it:
+                // FP16 holds p up to 2^15, and what lies 2^-20 below the largest p may lose bits.
+                const float tops = top * scale;
+                const bool move = tops - m > kLazy;
                 if (__any_sync(0xffffffffu, move)) {
-                    const float m_new = move ? top : m;
-                    const float alpha = move ? ex2((m - m_new) * scale) : 1.0f;
+                    const float m_new = move ? tops + kAhead : m;
+                    const float alpha = move ? ex2(m - m_new) : 1.0f;
                     m = m_new;
                     l *= alpha;
                     if (i > 0) {  // the accumulator follows (its last product is done: the scores came after it)
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                const float2 scale2 = make_float2(scale, scale), off2 = make_float2(-m * scale, -m * scale);
+                const float2 scale2 = make_float2(scale, scale), off2 = make_float2(-m, -m);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {  // 64 keys at a time: the first product starts under the second half
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
                 const size_t r = (static_cast<size_t>(sp) * p.T + token) * p.Hq + head;
-                if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(ok ? m * scale : kNegRef, ok ? l : 0.0f);
+                if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(ok ? m : kNegRef, ok ? l : 0.0f);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t v[32];
