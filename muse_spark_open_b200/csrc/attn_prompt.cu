@@ -18,8 +18,10 @@
 //                    FP16 over the scores.  The running reference m is set ahead of the maximum and moves only when a score
 //                    outgrows what FP16 holds, so the accumulator in TMEM is rescaled once or twice per row, not per tile
 //                    (800 clocks each time, in whichever warp has such a row).
-// The two row tiles take turns: while one's scores are exponentiated, the tensor cores work on the other's products.
-// TMEM: S (with P over its first half) and O, 128 columns each, for two row tiles = all 512 columns.
+// The products run ahead of the softmax in halves of 64 keys: while the softmax works on one half of a row tile's scores,
+// the tensor cores add the other half's product and put the next tile's scores in its place.  (With whole tiles each tile
+// waited 1300 clocks for its next scores, a third of the loop; a third row tile does not fit.)
+// TMEM: S (P over the first half of each half) and O, 128 columns each, for two row tiles = all 512 columns.
 // Pairs (CG = 2, tcgen05 cta_group::2): a tile's products run over both SMs, 256 rows, each CTA bringing its rows and half of
 // the K and V tile.  A single CTA is bound by shared memory: per tile 128 KB of Q and K reads, 64 KB of V, 96 KB of
 // conversion and 32 KB of TMA writes take 2560 clocks at 128 bytes each, the products 2048; a pair's CTA moves 192 KB.
@@ -43,6 +45,10 @@ struct Geo {
     static constexpr int kF8 = 16384 / CG;
     static constexpr int kKeys = kTile / CG;            // K rows here
     static constexpr int kChan = 128 / CG;              // V channels here
+    // Half a tile's scores: 64 columns.  Of a pair, each CTA brings 32 keys: columns 0 .. 31 are keys 32 half .. , columns
+    // 32 .. 63 the keys 64 further.  A single CTA takes 64 keys in a row.
+    static constexpr int kHalf = 64 / CG;               // keys between the first columns of the two halves
+    static constexpr int kNext = 32 * CG;               // keys between column 0 and column 32
     static constexpr int kSmem = 2 * kQBytes + 2 * kSlots * kF16 + 2 * kStages * kF8 + 1024;
 };
 static_assert(Geo<1>::kSmem <= 231000 && Geo<2>::kSmem <= 231000, "shared memory");
@@ -259,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using G = Geo<CG>;
     constexpr int NS = G::kSlots, SS = G::kStages;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[4 * SS + 4 * NS + 11];
+    __shared__ __align__(8) uint64_t bars[4 * SS + 4 * NS + 14];
     __shared__ uint32_t tmem_slot;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -274,11 +280,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* g_v = g_k + NS * G::kF16;
     uint8_t* g_f8 = g_v + NS * G::kF16;
     auto bar = [&](int i) { return smem_u32(&bars[i]); };
-    // staging full / free, K stages then V stages; operand slots full / free, K then V; queries; output; scores per row
-    // tile; halves of P per row tile.  With a pair, "full", "queries" and "P" collect both CTAs' arrivals at the even CTA;
+    // staging full / free, K stages then V stages; operand slots full / free, K then V; queries; output; halves of the
+    // scores and of P per row tile; products added per row tile.  With a pair, "full", "queries" and "P" collect both CTAs' arrivals at the even CTA;
     // what the MMAs signal arrives in both.
     const uint32_t st_full = bar(0), st_free = bar(2 * SS), op_full = bar(4 * SS), op_free = bar(4 * SS + 2 * NS),
-                   q_here = bar(4 * SS + 4 * NS), q_full = q_here + 8, o_done = q_here + 16, s_done = q_here + 32, p_ready = q_here + 48;
+                   q_here = bar(4 * SS + 4 * NS), q_full = q_here + 8, o_done = q_here + 16, s_done = q_here + 32, p_ready = q_here + 64,
+                   pv_done = q_here + 96;
     auto arrive_issuer = [&](uint32_t b) {
         if constexpr (CG == 1) mbar_arrive(b);
         else mbar_arrive_cluster(dsmem_addr(b, 0));
@@ -287,8 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 32) {
         for (int i = 0; i < 2 * SS; ++i) mbar_init(st_full + 8 * i, 1), mbar_init(st_free + 8 * i, 4);
         for (int i = 0; i < 2 * NS; ++i) mbar_init(op_full + 8 * i, 4 * CG), mbar_init(op_free + 8 * i, 1);
-        for (int i = 0; i < 2; ++i) mbar_init(o_done + 8 * i, 1), mbar_init(s_done + 8 * i, 1);
-        for (int i = 0; i < 4; ++i) mbar_init(p_ready + 8 * i, 4 * CG);
+        for (int i = 0; i < 2; ++i) mbar_init(o_done + 8 * i, 1), mbar_init(pv_done + 8 * i, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(s_done + 8 * i, 1), mbar_init(p_ready + 8 * i, 4 * CG);
         mbar_init(q_here, 1);
         mbar_init(q_full, CG);
         fence_mbar_init();
@@ -323,7 +330,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < 8) {
         // ================ softmax: thread = row of row tile g
-        reg_inc<192>();
         const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
         const int g = warp >> 2, row = tid & 127, j = tok_of(g) + (row >> 3), head = h * 8 + (row & 7);
         const int pos = p_first + j;
@@ -336,19 +342,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = kNegRef, l = 0.0f;
         bool ok = true;
         if ((g == 0 || two) && nt > 0) {
-            for (int i = 0; i < nt; ++i) {
-                ok = mbar_wait(s_done + 8 * g, i & 1, p.status, where | 3) && ok;
+            for (int t = 0; t < 2 * nt; ++t) {  // 64 keys at a time
+                const int half = t & 1, par = (t >> 1) & 1;
+                const uint32_t t_x = t_s + 64 * half;
+                ok = mbar_wait(s_done + 16 * g + 8 * half, par, p.status, where | 3) && ok;
                 tc_fence_after();
-                const int s0 = base_of(i);
-                uint32_t x[4][32];
+                uint32_t x[2][32];
+                float mx[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, x[c]);
+                for (int c = 0; c < 2; ++c) tmem_ld32(t_x + 32 * c, x[c]);
                 tmem_wait_ld();
-                if (s0 + kTile - 1 > g_first || (W > 0 && s0 <= g_last - W && s0 + kTile > snk)) {
+                const int s0 = base_of(t >> 1) + G::kHalf * half;  // position of the first key; the second 32 lie kNext further
+                if (s0 + G::kNext + 31 > g_first || (W > 0 && s0 <= g_last - W && s0 + G::kNext + 32 > snk)) {
                     // an edge of what the rows see: one bit per key
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int at = s0 + 32 * c;
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = s0 + G::kNext * c;
                         uint32_t vis = low_bits(pos - at + 1);
                         if (W > 0) vis &= ~low_bits(pos - W - at + 1) | low_bits(snk - at);
 #pragma unroll
@@ -356,26 +365,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (!(vis & (1u << e))) x[c][e] = 0xff800000u;  // -inf
                     }
                 }
-                float mx[8];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < 4; ++c) {
                     auto v = [&](int e) { return __uint_as_float(x[c >> 1][16 * (c & 1) + e]); };
                     mx[c] = max3(v(0), v(1), v(2));
 #pragma unroll
                     for (int e = 3; e < 15; e += 2) mx[c] = max3(mx[c], v(e), v(e + 1));
                     mx[c] = fmaxf(mx[c], v(15));
                 }
-                const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
                 // A new reference lies 2^kAhead above the row's maximum and serves until a score lies 2^kLazy above it:
                 // FP16 holds p up to 2^15, and what lies 2^-20 below the largest p may lose bits.
-                const float tops = top * scale;
+                const float tops = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
                 const bool move = tops - m > kLazy;
                 if (__any_sync(0xffffffffu, move)) {
                     const float m_new = move ? tops + kAhead : m;
                     const float alpha = move ? ex2(m - m_new) : 1.0f;
                     m = m_new;
                     l *= alpha;
-                    if (i > 0) {  // the accumulator follows (its last product is done: the scores came after it)
+                    if (t > 0) {  // the accumulator follows, once the last product has been added
+                        ok = mbar_wait(pv_done + 8 * g, (t - 1) & 1, p.status, where | 2) && ok;
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < 128; c += 16) {
                             uint32_t o[16];
@@ -389,23 +398,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const float2 scale2 = make_float2(scale, scale), off2 = make_float2(-m, -m);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                uint32_t w[32];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {  // 64 keys at a time: the first product starts under the second half
-                    uint32_t w[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int cc = 2 * half + (e >> 4), k = 2 * (e & 15);
-                        const float2 y = fma2(make_float2(__uint_as_float(x[cc][k]), __uint_as_float(x[cc][k + 1])), scale2, off2);
-                        const float2 v = e % kPolyEvery == kPolyEvery - 1 ? ex2_poly2(y) : make_float2(ex2(y.x), ex2(y.y));
-                        sum[e & 1] = add2(sum[e & 1], v);
-                        w[e] = pack_half(v.x, v.y);
-                    }
-                    tmem_st32(t_s + 32 * half, w);
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_issuer(p_ready + 16 * g + 8 * half);
+                for (int e = 0; e < 32; ++e) {
+                    const int cc = e >> 4, k = 2 * (e & 15);
+                    const float2 y = fma2(make_float2(__uint_as_float(x[cc][k]), __uint_as_float(x[cc][k + 1])), scale2, off2);
+                    const float2 v = e % kPolyEvery == kPolyEvery - 1 ? ex2_poly2(y) : make_float2(ex2(y.x), ex2(y.y));
+                    sum[e & 1] = add2(sum[e & 1], v);
+                    w[e] = pack_half(v.x, v.y);
                 }
+                tmem_st32(t_x, w);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_issuer(p_ready + 16 * g + 8 * half);
                 sum[0] = add2(sum[0], sum[1]);
                 l += sum[0].x + sum[0].y;
             }
@@ -481,7 +487,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp < 12) {
         // ================ converting: E4M3 staging -> FP16 operand tiles (this CTA's half of the keys of K, of the channels of V)
-        reg_dec<64>();
         const int w = warp - 8;
         bool ok = true;
         int stage = 0, st_ph = 0, slot = 0, op_ph = 0;
@@ -553,59 +558,69 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (++slot == NS) slot = 0, op_ph ^= 1;
         }
     } else {
-        reg_dec<64>();
         if (warp == 12) {
             // ================ the MMA warp: all lanes run the loop, one issues (of a pair, the even CTA's)
             if (nt > 0 && rank == 0) {
                 const uint32_t leader = elect_one();
-                const uint32_t id_qk = umma_idesc(128 * CG, 128, 0, 0, 0, 0), id_pv = umma_idesc(128 * CG, 128, 0, 0, 0, 1);
+                const uint32_t id_qk = umma_idesc(128 * CG, 64, 0, 0, 0, 0), id_pv = umma_idesc(128 * CG, 128, 0, 0, 0, 1);
                 const uint64_t d_q = umma_smem_desc(s_q, 16, 1024, kSwizzle128), d_k = umma_smem_desc(s_k, 16, 1024, kSwizzle128);
                 const uint64_t d_v = umma_smem_desc(s_v, 16384, 1024, kSwizzle128);
                 auto wait = [&](uint32_t b, int parity, int site) { return mbar_wait<0, (CG > 1)>(b, parity, p.status, where | site); };
-                auto scores = [&](int g, int slot) {  // S_g = Q_g K^T
+                auto scores = [&](int g, int slot, int half) {  // 64 keys' S_g = Q_g K^T
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t oq = ((e >> 2) * 16384 + (e & 3) * 32) >> 4, ok_ = ((e >> 2) * (G::kKeys * 128) + (e & 3) * 32) >> 4;
-                        umma_f16_ss_if<CG>(leader, tmem + g * 128, d_q + (g * kQBytes >> 4) + oq, d_k + (slot * G::kF16 >> 4) + ok_, id_qk, e != 0);
+                        umma_f16_ss_if<CG>(leader, tmem + g * 128 + 64 * half, d_q + (g * kQBytes >> 4) + oq,
+                                           d_k + ((slot * G::kF16 + half * G::kHalf * 128) >> 4) + ok_, id_qk, e != 0);
                     }
-                    umma_commit_if<CG>(leader, s_done + 8 * g);
+                    umma_commit_if<CG>(leader, s_done + 16 * g + 8 * half);
                 };
-                auto output = [&](int g, int slot, bool first, int par) {  // O_g (+)= P_g V, each half as soon as it is there
+                auto output = [&](int g, int slot, int half, bool first) {  // O_g (+)= P_g V over those 64 keys
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (!wait(p_ready + 16 * g + 8 * half, par, 10 + g)) return false;
-                        tc_fence_after();
-#pragma unroll
-                        for (int e = 4 * half; e < 4 * half + 4; ++e)
-                            umma_f16_ts_if<CG>(leader, tmem + 256 + g * 128, tmem + g * 128 + 8 * e, d_v + ((slot * G::kF16 + 2048 * e) >> 4), id_pv,
-                                               !first || e != 0);
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = half * G::kHalf + (e >> 1) * G::kNext + (e & 1) * 16;
+                        umma_f16_ts_if<CG>(leader, tmem + 256 + g * 128, tmem + g * 128 + 64 * half + 8 * e, d_v + ((slot * G::kF16 + row * 128) >> 4),
+                                           id_pv, !first || e != 0);
                     }
-                    return true;
+                    umma_commit_if<CG>(leader, pv_done + 8 * g);
                 };
                 bool ok = wait(q_full, 0, 7) && wait(op_full, 0, 8);
                 tc_fence_after();
                 if (ok) {
-                    scores(0, 0);
-                    if (two) scores(1, 0);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        scores(0, 0, half);
+                        if (two) scores(1, 0, half);
+                    }
                     umma_commit_if<CG>(leader, op_free);
                 }
                 int slot = 0, ph = 0;
                 for (int i = 0; i < nt && ok; ++i) {
                     const bool more = i + 1 < nt;
                     const int nslot = slot + 1 == NS ? 0 : slot + 1, nph = slot + 1 == NS ? ph ^ 1 : ph;
-                    ok = wait(op_full + 8 * (NS + slot), ph, 9) && output(0, slot, i == 0, i & 1);
-                    if (ok && more) {
-                        ok = wait(op_full + 8 * nslot, nph, 12);
-                        tc_fence_after();
-                        if (ok) scores(0, nslot);
+                    ok = wait(op_full + 8 * (NS + slot), ph, 9);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            if (g == 1 && !two) break;
+                            ok = ok && wait(p_ready + 16 * g + 8 * half, i & 1, 10 + g);
+                            if (!ok) break;
+                            tc_fence_after();
+                            output(g, slot, half, i == 0 && half == 0);
+                            if (more) {  // the next tile's scores over the probabilities just read
+                                if (half == 0 && g == 0) {
+                                    ok = wait(op_full + 8 * nslot, nph, 12);
+                                    if (!ok) break;
+                                    tc_fence_after();
+                                }
+                                scores(g, nslot, half);
+                            }
+                        }
                     }
-                    if (ok && two) ok = output(1, slot, i == 0, i & 1);
                     if (!ok) break;
                     umma_commit_if<CG>(leader, op_free + 8 * (NS + slot));
-                    if (more) {
-                        if (two) scores(1, nslot);
-                        umma_commit_if<CG>(leader, op_free + 8 * nslot);
-                    }
+                    if (more) umma_commit_if<CG>(leader, op_free + 8 * nslot);
                     slot = nslot, ph = nph;
                 }
                 umma_commit_if<CG>(leader, o_done);
