@@ -141,7 +141,7 @@ typedef struct {
     const float* k_scale;
     const float* v_scale;
     const int32_t* seq_lens;  /* [B] cached tokens per request */
-    const int32_t* cu_seqlens_q; /* [B + 1] rising, cu_seqlens_q[B] <= T */
+    const int32_t* cu_seqlens_q; /* [B + 1] rising, cu_seqlens_q[B] <= T; NULL: q_len tokens each, T = B * q_len */
     const int32_t* page_table;/* [B, max_pages] */
     int max_pages;
     const float* inv_freq;    /* [d/2] or NULL */
@@ -152,11 +152,12 @@ typedef struct {
     void* scratch;            /* msk_attn_prompt_scratch_bytes(), 256-byte aligned, any contents; launches that may overlap on
                                  the GPU need one each */
     size_t scratch_bytes;
+    int q_len;
 } MskPromptParams;
 
 int msk_attn_prompt(const MskPromptParams* p, int* status, void* stream);
 
-/* Bytes of the workspace for a call of that shape (B, T, heads, max_pages, page_size, window, sinks, splits are read). */
+/* Bytes of the workspace for a call of that shape (B, T, heads, max_pages, page_size, window, sinks, splits, cu_seqlens_q == NULL and q_len are read). */
 int msk_attn_prompt_scratch_bytes(const MskPromptParams* p, size_t* bytes);
 
 /* ---------------------------------------------------------------- pages of a paged cache

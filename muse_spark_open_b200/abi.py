@@ -202,7 +202,7 @@ class PromptParams(C.Structure):
         ("B", C.c_int), ("T", C.c_int), ("Hq", C.c_int), ("Hkv", C.c_int), ("d", C.c_int), ("page_size", C.c_int),
         ("num_pages", C.c_int), ("window", C.c_int), ("sinks", C.c_int),
         ("qk_scale_factor", C.c_float), ("sm_scale", C.c_float), ("splits", C.c_int), ("pdl", C.c_int),
-        ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t),
+        ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t), ("q_len", C.c_int),
     ]
 
 

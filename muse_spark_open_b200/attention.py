@@ -4,6 +4,8 @@
 muse_attention_decode/submission.py:37-65; the new tokens' K/V are written into
 `data["k_cache"]` / `data["v_cache"]` in place at `data["cache_loc"]`, like the reference.
 With a window, `config["sinks"]` (default 0) first positions stay visible to every token.
+q_len is 1 (decode) or 8 (verify) as in the reference, or any other length: blocks other than 1 and 8, and blocks of 8 with
+sinks, write the new rows where the page table says (cache_loc says the same in the reference, submission.py:37-65).
 Nothing derived from `data` is cached between calls; only the RoPE frequency table (a function of
 theta and head_dim) is kept per device.
 """
@@ -69,11 +71,74 @@ def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
     else:
         ld = qkv.view(b * l, -1).stride(0)
     out = torch.empty((b, l, wide), dtype=torch.bfloat16, device=qkv.device)
+    if l != 1 and (l != 8 or (cfg.get("sinks", 0) and cfg["window"])) and not chunks and not stages:
+        # blocks of other lengths, and verify blocks with sinks: the prompt kernels (16 requests x 8 tokens, window 1024 + 4
+        # sinks: VERIFY_NEW us against VERIFY_OLD us for the verify kernel, whose results without sinks stay what they were)
+        _run_prompt(data, cfg, qkv.view(b * l, -1) if ld != qkv.stride(0) else qkv, out.view(b * l, wide), None, l, 0)
+        return out
     _run_step(abi.ptr(qkv), ld, out.data_ptr(), wide, data, cfg, qkv.get_device(), chunks, stages, 0, False, 0)
     return out
 
 
 _prompt_bytes: dict = {}
+
+
+def _run_prompt(data: dict, cfg: dict, qkv: torch.Tensor, out: torch.Tensor | None, cu: torch.Tensor | None, q_len: int, splits: int) -> torch.Tensor:
+    """msk_attn_prompt on checked arguments; cu None: q_len tokens per request."""
+    kc, vc, table, seq, ks, vs = data["k_cache"], data["v_cache"], data["page_table"], data["seq_lens"], data["k_scale"], data["v_scale"]
+    b, hq, hkv, d, page = cfg["batch"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"], cfg["page_size"]
+    if qkv.dtype != torch.bfloat16 or kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
+        raise abi.MskError("qkv must be bfloat16 and the cache float8_e4m3fn")
+    t, wide = qkv.shape if qkv.dim() == 2 else (0, 0)
+    if wide < (2 * hq + 2 * hkv) * d or qkv.stride(1) != 1:
+        raise abi.MskError("qkv must be [tokens, (2Hq+2Hkv)*d] with unit column stride")
+    if seq.dtype != torch.int32 or table.dtype != torch.int32 or (cu is not None and cu.dtype != torch.int32):
+        raise abi.MskError("seq_lens / page_table / cu_seqlens_q must be int32")
+    if seq.numel() != b or table.dim() != 2 or table.shape[0] != b or not (seq.is_contiguous() and table.is_contiguous()) or \
+            (cu is not None and (cu.numel() != b + 1 or not cu.is_contiguous())):
+        raise abi.MskError("seq_lens [B], page_table [B, max_pages] and cu_seqlens_q [B + 1] must be contiguous")
+    pages = kc.shape[0]
+    shape = (pages, page, hkv, d)
+    if kc.shape != shape or vc.shape != shape or not (kc.is_contiguous() and vc.is_contiguous()):
+        raise abi.MskError("k_cache / v_cache must be contiguous [num_pages, page_size, Hkv, d]")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise abi.MskError("k_scale / v_scale must be float32")
+    index = abi.here((qkv, kc, vc, ks, vs, seq, table) if cu is None else (qkv, kc, vc, ks, vs, seq, table, cu))
+    dev = qkv.device
+    if out is None:
+        out = torch.empty((t, hq * d), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.shape != (t, hq * d) or out.stride(1) != 1:
+        raise abi.MskError("out must be bfloat16 [tokens, Hq*d] with unit column stride")
+    elif out.get_device() != index:
+        raise abi.MskError("the tensors of one call must be on one device")
+    if t == 0:
+        return out
+    theta, window, sinks, max_pages = cfg["rope_theta"], cfg["window"], cfg.get("sinks", 0), table.shape[1]
+    freq = 0
+    if theta:
+        f = _inv_freq.get((float(theta), d, index))
+        freq = (inv_freq(theta, d, dev) if f is None else f).data_ptr()
+    lib = abi.lib()
+    # the workspace's size is a function of sizes alone
+    key = (b, t, hq, hkv, d, page, pages, window, sinks, max_pages, splits, q_len)
+    nbytes = _prompt_bytes.get(key)
+    if nbytes is None:
+        n = C.c_size_t()
+        p = abi.PromptParams(B=b, T=t, Hq=hq, Hkv=hkv, d=d, page_size=page, num_pages=pages, window=window, sinks=sinks, max_pages=max_pages,
+                             splits=splits, q_len=q_len, cu_seqlens_q=None if cu is None else cu.data_ptr())
+        abi.check(lib.msk_attn_prompt_scratch_bytes(C.byref(p), C.byref(n)), "msk_attn_prompt_scratch_bytes")
+        if len(_prompt_bytes) > 4096:
+            _prompt_bytes.clear()
+        nbytes = _prompt_bytes[key] = n.value
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    args = _prompt_args.pack(
+        qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), seq.data_ptr(),
+        0 if cu is None else cu.data_ptr(), table.data_ptr(), max_pages, freq, b, t, hq, hkv, d, page, pages, window, sinks,
+        cfg["qk_scale_factor"], cfg["sm_scale"], splits, 0, scratch.data_ptr(), nbytes, q_len)
+    rc = lib.msk_attn_prompt(args, abi.status_ptr(index), abi.raw_stream(index))
+    if rc:
+        abi.check(rc, "msk_attn_prompt")
+    return out
 
 
 def prompt_fn(data: dict, out: torch.Tensor | None = None, splits: int = 0) -> torch.Tensor:
@@ -85,54 +150,4 @@ def prompt_fn(data: dict, out: torch.Tensor | None = None, splits: int = 0) -> t
     (a padded batch) are not touched: they keep what `out` held.  The workspace comes from torch's allocator on the current
     stream, so calls on several streams or in several captured graphs do not share it.
     """
-    cfg, qkv, kc, vc = data["config"], data["qkv"], data["k_cache"], data["v_cache"]
-    table, seq, cu, ks, vs = data["page_table"], data["seq_lens"], data["cu_seqlens_q"], data["k_scale"], data["v_scale"]
-    b, hq, hkv, d, page = cfg["batch"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"], cfg["page_size"]
-    if qkv.dtype != torch.bfloat16 or kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
-        raise abi.MskError("qkv must be bfloat16 and the cache float8_e4m3fn")
-    t, wide = qkv.shape if qkv.dim() == 2 else (0, 0)
-    if wide < (2 * hq + 2 * hkv) * d or qkv.stride(1) != 1:
-        raise abi.MskError("qkv must be [tokens, (2Hq+2Hkv)*d] with unit column stride")
-    if seq.dtype != torch.int32 or table.dtype != torch.int32 or cu.dtype != torch.int32:
-        raise abi.MskError("seq_lens / page_table / cu_seqlens_q must be int32")
-    if seq.numel() != b or table.dim() != 2 or table.shape[0] != b or cu.numel() != b + 1 or \
-            not (seq.is_contiguous() and table.is_contiguous() and cu.is_contiguous()):
-        raise abi.MskError("seq_lens [B], page_table [B, max_pages] and cu_seqlens_q [B + 1] must be contiguous")
-    shape = (kc.shape[0], page, hkv, d)
-    if kc.shape != shape or vc.shape != shape or not (kc.is_contiguous() and vc.is_contiguous()):
-        raise abi.MskError("k_cache / v_cache must be contiguous [num_pages, page_size, Hkv, d]")
-    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
-        raise abi.MskError("k_scale / v_scale must be float32")
-    index = abi.here((qkv, kc, vc, ks, vs, seq, cu, table))
-    dev = qkv.device
-    if out is None:
-        out = torch.empty((t, hq * d), dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.shape != (t, hq * d) or out.stride(1) != 1:
-        raise abi.MskError("out must be bfloat16 [tokens, Hq*d] with unit column stride")
-    else:
-        abi.here((qkv, out))
-    if t == 0:
-        return out
-    theta, window, sinks, max_pages = cfg["rope_theta"], cfg["window"], cfg.get("sinks", 0), table.shape[1]
-    freq = inv_freq(theta, d, dev) if theta else None
-    lib = abi.lib()
-    # the workspace's size is a function of sizes alone
-    key = (b, t, hq, hkv, d, page, kc.shape[0], window, sinks, max_pages, splits)
-    nbytes = _prompt_bytes.get(key)
-    if nbytes is None:
-        n = C.c_size_t()
-        p = abi.PromptParams(B=b, T=t, Hq=hq, Hkv=hkv, d=d, page_size=page, num_pages=kc.shape[0], window=window, sinks=sinks, max_pages=max_pages,
-                             splits=splits)
-        abi.check(lib.msk_attn_prompt_scratch_bytes(C.byref(p), C.byref(n)), "msk_attn_prompt_scratch_bytes")
-        if len(_prompt_bytes) > 4096:
-            _prompt_bytes.clear()
-        nbytes = _prompt_bytes[key] = n.value
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args = _prompt_args.pack(
-        qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), seq.data_ptr(),
-        cu.data_ptr(), table.data_ptr(), max_pages, freq.data_ptr() if freq is not None else 0, b, t, hq, hkv, d, page, kc.shape[0], window, sinks,
-        cfg["qk_scale_factor"], cfg["sm_scale"], splits, 0, scratch.data_ptr(), nbytes)
-    rc = lib.msk_attn_prompt(args, abi.status_ptr(index), abi.raw_stream(index))
-    if rc:
-        abi.check(rc, "msk_attn_prompt")
-    return out
+    return _run_prompt(data, data["config"], data["qkv"], out, data["cu_seqlens_q"], 0, splits)

@@ -69,7 +69,8 @@ struct PromptArgs {
     const float* k_scale;
     const float* v_scale;
     const int* seq_lens;
-    const int* cu;
+    const int* cu;    // or NULL: q_len tokens each
+    int q_len;
     const int* page_table;
     int max_pages;
     const float* inv_freq;
@@ -79,15 +80,16 @@ struct PromptArgs {
     __half* q16;      // [T, Hq, 128]
     int* units;       // [kMaxUnitsHeader + 4 * max_units]: request, first row of qkv, tokens, first position
     int unit;         // tokens per unit
+    int direct;       // the main kernel finds its unit itself (few requests, one wave: the order does not matter)
     float* part_o;    // [splits, T * Hq, 128]
     float* part_ml;   // [splits, T * Hq, 2]
     int* status;
 };
 
-__device__ __forceinline__ int new_tokens(const PromptArgs& p, int b) {
-    const int lo = min(max(p.cu[b], 0), p.T), hi = min(max(p.cu[b + 1], 0), p.T);
-    return max(hi - lo, 0);
+__device__ __forceinline__ int first_row(const PromptArgs& p, int b) {  // of qkv and out; b = B: the end
+    return p.cu != nullptr ? min(max(p.cu[b], 0), p.T) : b * p.q_len;
 }
+__device__ __forceinline__ int new_tokens(const PromptArgs& p, int b) { return max(first_row(p, b + 1) - first_row(p, b), 0); }
 
 // RMSNorm (weightless, eps 1e-5), scale and interleaved RoPE of one 128-wide head row, 4 values per lane.
 __device__ __forceinline__ void norm_turn(float (&x)[4], float post_scale, const float (&c)[2], const float (&s)[2], bool turn) {
@@ -126,7 +128,7 @@ __device__ void list_units(const PromptArgs& p) {
         for (int b0 = 0; b0 < p.B; b0 += 256) {
             __syncthreads();
             const int b = b0 + tid;
-            if (b < p.B) n_s[tid] = new_tokens(p, b), seq_s[tid] = p.seq_lens[b], row_s[tid] = min(max(p.cu[b], 0), p.T);
+            if (b < p.B) n_s[tid] = new_tokens(p, b), seq_s[tid] = p.seq_lens[b], row_s[tid] = first_row(p, b);
             __syncthreads();
             for (int r = warp; r < 256 && b0 + r < p.B; r += 8) {
                 const int n = n_s[r], units = (n + p.unit - 1) / p.unit;
@@ -168,15 +170,30 @@ __device__ void list_units(const PromptArgs& p) {
 __global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
     pdl_wait();
     pdl_launch_dependents();
-    const int t = blockIdx.x;
-    if (t == p.T) {
+    if (blockIdx.x == 0 && !p.direct) {  // first, it takes longest
         list_units(p);
         return;
     }
+    const int t = blockIdx.x - (p.direct ? 0 : 1);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // everything that needs no look-up is asked for first: the token's head rows, the frequencies, the scales
+    const __nv_bfloat16* row = p.qkv + static_cast<size_t>(t) * p.ld_qkv;
+    const int heads = p.Hq + 2 * p.Hkv;
+    constexpr int U = 5;  // rows in flight per warp: 8 warps cover 40 heads at once
+    uint2 raw[U];
+    auto fetch = [&](int h0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (h0 + 8 * u < heads) raw[u] = __ldg(reinterpret_cast<const uint2*>(row + (h0 + 8 * u) * 128 + 4 * lane));
+    };
+    fetch(warp);
+    const bool turn = p.inv_freq != nullptr;
+    const float2 freq = turn ? __ldg(reinterpret_cast<const float2*>(p.inv_freq) + lane) : make_float2(0.0f, 0.0f);
+    const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
     // the request of token t: the last b with cu[b] <= t, by steps of 32 requests
     int lo = 0, hi = p.B;  // cu[lo] <= t < cu[hi] is looked for in [lo, hi)
-    if (t >= p.cu[p.B] || t < p.cu[0]) return;  // a row behind the last sequence
+    if (p.cu == nullptr) lo = t / p.q_len, hi = lo + 1;
+    else if (t >= p.cu[p.B] || t < p.cu[0]) return;  // a row behind the last sequence
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, at = lo + step * lane;
         const bool le = at < hi && p.cu[at] <= t;
@@ -186,35 +203,27 @@ __global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
         lo = nlo;
     }
     const int b = lo;
-    const int pos = p.seq_lens[b] + t - p.cu[b];
+    const int pos = p.seq_lens[b] + t - (p.cu != nullptr ? p.cu[b] : b * p.q_len);
     float c[2] = {1.0f, 1.0f}, s[2] = {0.0f, 0.0f};
-    const bool turn = p.inv_freq != nullptr;
     if (turn) {
         const float fp = static_cast<float>(pos);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             // the product's rounding error (up to 5e-4 at position 8192) is put back to first order
-            const float f = p.inv_freq[2 * lane + h], ang = fp * f, err = fmaf(fp, f, -ang);
+            const float f = h ? freq.y : freq.x, ang = fp * f, err = fmaf(fp, f, -ang);
             float cs, sn;
             sincosf(ang, &sn, &cs);
             c[h] = cs - err * sn;
             s[h] = sn + err * cs;
         }
     }
-    const __nv_bfloat16* row = p.qkv + static_cast<size_t>(t) * p.ld_qkv;
-    const int heads = p.Hq + 2 * p.Hkv;
     const int page = pos >> p.page_log;
     const int id = pos >= 0 && page < p.max_pages ? p.page_table[static_cast<size_t>(b) * p.max_pages + page] : -1;
     const bool page_ok = id >= 0 && id < p.num_pages;
     if (!page_ok && threadIdx.x == 0) report(p.status, MSK_ERR_BOUNDS, MSK_K_PROMPT << 8 | 2, id, page);
-    const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
     const size_t slot = page_ok ? (static_cast<size_t>(id) << p.page_log) + (pos & (p.page_size - 1)) : 0;
-    constexpr int U = 5;  // rows in flight per warp: 8 warps cover 40 heads at once
     for (int h0 = warp; h0 < heads; h0 += 8 * U) {
-        uint2 raw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (h0 + 8 * u < heads) raw[u] = *reinterpret_cast<const uint2*>(row + (h0 + 8 * u) * 128 + 4 * lane);
+        if (h0 != warp) fetch(h0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = h0 + 8 * u;
@@ -306,9 +315,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_launch_dependents();
 
     // ---------------- this CTA's unit: the pair's row tile g covers tokens 16 CG g .. of the unit, this CTA 16 of them
-    const int n_units = __ldcg(p.units);
-    int4 u = make_int4(0, 0, 0, 0);
-    if (slot_u < n_units) u = __ldcg(reinterpret_cast<const int4*>(p.units + kMaxUnitsHeader + 4 * slot_u));
+    int4 u = make_int4(0, 0, 0, 0);  // request, first row, tokens, first position
+    if (!p.direct) {
+        const int n_units = __ldcg(p.units);
+        if (slot_u < n_units) u = __ldcg(reinterpret_cast<const int4*>(p.units + kMaxUnitsHeader + 4 * slot_u));
+    } else if (p.cu == nullptr) {
+        const int per_req = (p.q_len + p.unit - 1) / p.unit, rb = slot_u / per_req, at = (slot_u - rb * per_req) * p.unit;
+        if (rb < p.B) u = make_int4(rb, rb * p.q_len + at, min(p.q_len - at, p.unit), p.seq_lens[rb] + at);
+    } else {  // a lane per request (B <= 32): which one's groups of tokens hold number slot_u
+        const int n = lane < p.B ? new_tokens(p, lane) : 0, row0 = lane < p.B ? first_row(p, lane) : 0, seq = lane < p.B ? p.seq_lens[lane] : 0;
+        const int groups = (n + p.unit - 1) / p.unit;
+        int inc = groups;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, inc > slot_u);
+        if (behind != 0) {
+            const int src = __ffs(behind) - 1;
+            const int at = (slot_u - (__shfl_sync(0xffffffffu, inc, src) - __shfl_sync(0xffffffffu, groups, src))) * p.unit;
+            u = make_int4(src, __shfl_sync(0xffffffffu, row0, src) + at, min(__shfl_sync(0xffffffffu, n, src) - at, p.unit),
+                          __shfl_sync(0xffffffffu, seq, src) + at);
+        }
+    }
     const int b = u.x, tok0 = u.y, n_tok = u.z, p_first = u.w, p_last = p_first + max(n_tok, 1) - 1;
     const int W = p.window, snk = W > 0 ? p.sinks : 0;
     int t_first, sink_tiles;
@@ -694,8 +724,7 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(PromptArgs p) {
     const int lane = threadIdx.x & 31;
     const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     const int token = static_cast<int>(row / p.Hq), head = static_cast<int>(row % p.Hq);
-    const int last = min(p.cu[p.B], p.T);
-    if (token >= last || token < p.cu[0]) return;
+    if (token >= first_row(p, p.B) || token < first_row(p, 0)) return;
     const size_t stride = static_cast<size_t>(p.T) * p.Hq;
     float m = kNegRef;
     for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (s * stride + row)]);
@@ -736,7 +765,9 @@ int plan_prompt(const MskPromptParams* q, Plan* plan) {
     // Pairs of CTAs where requests bring more than 32 tokens on average: a unit of 64 tokens then fills both.
     plan->cg = static_cast<long long>(q->T) > 32ll * q->B ? 2 : 1;
     const int unit = 2 * kTok * plan->cg;
-    const long long units = static_cast<long long>(q->T) / unit + q->B;  // sum of ceil(n / unit) is at most this
+    const long long units = q->cu_seqlens_q == nullptr && q->q_len > 0
+                                ? static_cast<long long>(q->B) * ((q->q_len + unit - 1) / unit)
+                                : static_cast<long long>(q->T) / unit + q->B;  // sum of ceil(n / unit) is at most this
     plan->max_units = static_cast<int>(units < q->T ? units : q->T);
     long long tiles = (static_cast<long long>(q->max_pages) * q->page_size + kTile - 1) / kTile;
     if (q->window > 0) {
@@ -777,8 +808,9 @@ extern "C" int msk_attn_prompt_scratch_bytes(const MskPromptParams* q, size_t* b
 extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stream) {
     using namespace msk;
     if (q == nullptr || !q->qkv || !q->out || !q->k_cache || !q->v_cache || !q->k_scale || !q->v_scale || !q->seq_lens ||
-        !q->cu_seqlens_q || !q->page_table || !q->scratch)
+        !q->page_table || !q->scratch)
         return MSK_ERR_INVALID;
+    if (q->cu_seqlens_q == nullptr && (q->q_len < 1 || static_cast<long long>(q->B) * q->q_len != q->T)) return MSK_ERR_INVALID;
     Plan plan;
     int rc = plan_prompt(q, &plan);
     if (rc != 0) return rc;
@@ -797,7 +829,7 @@ extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stre
     a.qkv = static_cast<const __nv_bfloat16*>(q->qkv), a.ld_qkv = q->ld_qkv;
     a.out = static_cast<__nv_bfloat16*>(q->out), a.ld_out = q->ld_out;
     a.k_cache = static_cast<uint8_t*>(q->k_cache), a.v_cache = static_cast<uint8_t*>(q->v_cache);
-    a.k_scale = q->k_scale, a.v_scale = q->v_scale, a.seq_lens = q->seq_lens, a.cu = q->cu_seqlens_q;
+    a.k_scale = q->k_scale, a.v_scale = q->v_scale, a.seq_lens = q->seq_lens, a.cu = q->cu_seqlens_q, a.q_len = q->q_len;
     a.page_table = q->page_table, a.max_pages = q->max_pages, a.inv_freq = q->inv_freq;
     a.B = q->B, a.T = q->T, a.Hq = q->Hq, a.Hkv = q->Hkv, a.page_size = q->page_size, a.num_pages = q->num_pages;
     while ((1 << a.page_log) < q->page_size) ++a.page_log;
@@ -810,6 +842,7 @@ extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stre
     while (qs * 2.0f * qmax <= 32768.0f && qs < 65536.0f) qs *= 2.0f;
     while (qs * qmax > 32768.0f && qs > 1.0f / 65536.0f) qs *= 0.5f;
     a.q_scale = qs, a.s_scale = q->sm_scale * 1.4426950408889634f / qs;
+    a.direct = ctas <= 148 && (q->cu_seqlens_q == nullptr || q->B <= 32);
     a.q16 = reinterpret_cast<__half*>(ws + plan.q16), a.units = reinterpret_cast<int*>(ws + plan.units);
     a.part_ml = reinterpret_cast<float*>(ws + plan.ml), a.part_o = reinterpret_cast<float*>(ws + plan.o);
     a.status = status;
@@ -849,7 +882,7 @@ extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stre
     cudaLaunchConfig_t cfg = {};
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
-    cfg.gridDim = dim3(q->T + 1), cfg.blockDim = dim3(256), cfg.numAttrs = q->pdl ? 1 : 0;
+    cfg.gridDim = dim3(q->T + (a.direct ? 0 : 1)), cfg.blockDim = dim3(256), cfg.numAttrs = q->pdl ? 1 : 0;
     if (cudaLaunchKernelEx(&cfg, prompt_prep_kernel, a) != cudaSuccess) return MSK_ERR_CUDA;
     cfg.gridDim = dim3(static_cast<unsigned>(ctas)), cfg.blockDim = dim3(kThreads), cfg.numAttrs = 2;
     cfg.dynamicSmemBytes = plan.cg == 2 ? Geo<2>::kSmem : Geo<1>::kSmem;
