@@ -6,10 +6,11 @@
 // ones, in the order of the calls' rows, so that results do not depend on scheduling.  No call reads anything back to the
 // host: all of them can be captured.
 //
-// Allocation and compaction need ranks over `refs` (the k-th free page): one cluster of eight CTAs counts its slices,
-// exchanges the counts, and ranks (two reads of 4 bytes per page; a single CTA would take 4 times as long at 65536 pages,
-// a grid-wide scan a second launch).  What follows -- table rows, page data -- is a second launch over all SMs, chained
-// programmatically.  Bound by latency at small sizes, by memory (page data, read once and written once) at large ones.
+// Allocation and compaction need ranks over `refs` (the k-th free page): every warp counts a contiguous slice, the counts are
+// exchanged, and the slices are walked again with the ranks known.  Up to kOneCta pages one CTA does it (its barriers cost 30
+// ns), beyond a cluster of eight (1.2 us per exchange, eight times the loads in flight).  What follows -- table rows, page
+// data -- is a second launch over all SMs, chained programmatically.  Bound by latency at small sizes, by memory (page data,
+// read once and written once) at large ones.
 #include "msk.h"
 #include "ptx.cuh"
 
@@ -19,6 +20,7 @@ namespace {
 constexpr int kCluster = 8;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kOneCta = 16384;        // pages (free + extend of 16 rows, one CTA / cluster: 4096 pages 9.2 / 13.0 us, 65536 18.6 / 13.8)
 constexpr int kCopyThreads = 256;
 constexpr int kCopyChunk = 16384;     // bytes a CTA moves at a time: 4 x 16 per thread in flight
 constexpr int kMaxCaches = 128;
@@ -43,7 +45,7 @@ struct PlanArgs {
     int tokens;            // entries of cache_loc
     long long* cache_loc;
     // workspace
-    int* counts;           // [3][kCluster] slices' counts, then [4]: results
+    int* counts;           // [3][kCluster * kPlanWarps] slices' counts, then [4]: results
     int* claim;            // [rows] first list entry that names a row
     int* is_parent;        // [rows]
     int* need;             // [n]
@@ -82,17 +84,23 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
     return before + inc - v;
 }
 
-__device__ __forceinline__ void cluster_exchange() {  // everything written so far, global memory included, is visible after it
-    __threadfence();
-    cluster_sync_all();
+// Everything written so far, global memory included, is visible to all planning threads after it.
+__device__ __forceinline__ void exchange(int nct) {
+    if (nct == 1) {
+        __syncthreads();
+    } else {
+        __threadfence();
+        cluster_sync_all();
+    }
 }
 
-// Walks the pages [lo, hi) of `refs`, four per thread and step: f(first page, r[4], how many) for every thread and step
-// (the same number of steps for every thread).
+// Walks the pages [lo, hi) of `refs` with one warp, four per lane and step: f(first page, r[4], how many).
 template <class F>
 __device__ __forceinline__ void walk_refs(const int* refs, int lo, int hi, F f) {
-    for (int at = lo; at < hi; at += 4 * kPlanThreads) {
-        const int i = at + 4 * static_cast<int>(threadIdx.x);
+    const int lane = threadIdx.x & 31;
+#pragma unroll 4
+    for (int at = lo; at < hi; at += 128) {
+        const int i = at + 4 * lane;
         int r[4] = {0, 0, 0, 0};
         const int k = min(max(hi - i, 0), 4);
         if (k == 4 && (reinterpret_cast<uintptr_t>(refs + i) & 15) == 0) {
@@ -105,21 +113,34 @@ __device__ __forceinline__ void walk_refs(const int* refs, int lo, int hi, F f) 
     }
 }
 
-__device__ __forceinline__ void slice_of(const PlanArgs& p, int rank, int* lo, int* hi) {  // multiples of four pages
-    const int per = ((p.num_pages + kCluster - 1) / kCluster + 3) & ~3;
-    *lo = min(rank * per, p.num_pages);
-    *hi = min(*lo + per, p.num_pages);
+__device__ __forceinline__ void slice_of(const PlanArgs& p, int gwarp, int nwarps, int* lo, int* hi) {  // multiples of a step
+    const int per = ((p.num_pages + nwarps - 1) / nwarps + 127) & ~127;
+    *lo = static_cast<int>(min(static_cast<long long>(gwarp) * per, static_cast<long long>(p.num_pages)));
+    *hi = static_cast<int>(min(static_cast<long long>(*lo) + per, static_cast<long long>(p.num_pages)));
 }
 
-__device__ __forceinline__ int slice_total(const int* counts, int rank, int* before) {
-    int total = 0;
-    *before = 0;
-    for (int r = 0; r < kCluster; ++r) {
-        const int v = __ldcg(counts + r);
-        if (r < rank) *before += v;
-        total += v;
+__device__ __forceinline__ int warp_total(int v) { return __reduce_add_sync(0xffffffffu, v); }
+__device__ __forceinline__ int lanes_before(int v) {  // sum over the lower lanes
+    const int lane = threadIdx.x & 31;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
     }
-    return total;
+    return inc - v;
+}
+// (sum of the counts of all slices, of those before slice gwarp) -- a whole warp.
+__device__ __forceinline__ int slice_total(const int* counts, int gwarp, int nwarps, int* before) {
+    const int lane = threadIdx.x & 31;
+    int all = 0, low = 0;
+    for (int w = lane; w < nwarps; w += 32) {
+        const int v = __ldcg(counts + w);
+        all += v;
+        if (w < gwarp) low += v;
+    }
+    *before = warp_total(low);
+    return warp_total(all);
 }
 
 // The new tokens of list entry j: [first logical page, last] of row; tokens.
@@ -133,13 +154,13 @@ __device__ __forceinline__ void span_of(const PlanArgs& p, int row, int j, int* 
     }
 }
 
-// One cluster: gives list entries the free pages they need.  kFork: one page for a child whose parent ends inside a page.
+// One CTA or one cluster: gives list entries the free pages they need.  kFork: one page for a child whose parent ends inside a page.
 template <bool kFork>
-__global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1) pages_plan_kernel(PlanArgs p) {
+__global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int rank = static_cast<int>(cluster_ctarank());
+    const int rank = blockIdx.x, nct = gridDim.x;  // one CTA, or the one cluster
     const int gtid = rank * kPlanThreads + tid, gwarp = rank * kPlanWarps + warp;
-    constexpr int kAll = kCluster * kPlanThreads, kAllWarps = kCluster * kPlanWarps;
+    const int kAll = nct * kPlanThreads, kAllWarps = nct * kPlanWarps;
     pdl_wait();
     pdl_launch_dependents();
     // which list entry speaks for a row: the first that names it
@@ -148,15 +169,14 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
         if (kFork) p.is_parent[r] = 0;
     }
     int lo, hi;
-    slice_of(p, rank, &lo, &hi);
+    slice_of(p, gwarp, kAllWarps, &lo, &hi);
     int mine = 0;
     walk_refs(p.refs, lo, hi, [&](int, const int (&r)[4], int k) {
         for (int j = 0; j < 4; ++j) mine += j < k && r[j] == 0;
     });
-    int slice_free;
-    block_scan(mine, &slice_free);
-    if (tid == 0) p.counts[rank] = slice_free;
-    cluster_exchange();
+    mine = warp_total(mine);
+    if (lane == 0) p.counts[gwarp] = mine;
+    exchange(nct);
     for (int j = gtid; j < p.n; j += kAll) {
         const int row = p.list[j];
         if (row >= 0 && row < p.rows) atomicMin(p.claim + row, j);
@@ -165,35 +185,50 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
             if (par >= 0 && par < p.rows) atomicExch(p.is_parent + par, 1);
         }
     }
-    cluster_exchange();
-    // what each entry needs: a warp per entry, a lane per page
-    for (int j = gwarp; j < p.n; j += kAllWarps) {
-        const int row = p.list[j];
-        bool ok = row >= 0 && row < p.rows && __ldcg(p.claim + row) == j;
-        int need = 0;
-        if (kFork) {
-            const int par = p.parents[j];
-            ok = ok && par >= 0 && par < p.rows && __ldcg(p.is_parent + row) == 0;
-            if (lane == 0) {
+    exchange(nct);
+    // what each entry needs: a thread per entry where it is few pages, else a warp per entry and a lane per page
+    const bool few = kFork || (p.cu == nullptr && p.q_len <= 4 * p.page_size);
+    if (few) {
+        for (int j = gtid; j < p.n; j += kAll) {
+            const int row = p.list[j];
+            bool ok = row >= 0 && row < p.rows && __ldcg(p.claim + row) == j;
+            int need = 0;
+            if (kFork) {
+                const int par = p.parents[j];
+                ok = ok && par >= 0 && par < p.rows && __ldcg(p.is_parent + row) == 0;
                 int4 op = make_int4(-1, -1, 0, 0);
                 if (ok) {
                     const int seq = max(p.seq_lens[par], 0), full = seq >> p.page_log, part = seq & (p.page_size - 1);
-                    op.w = 1;
-                    if (full + (part > 0) > p.max_pages) {
-                        op.w = 0;
-                        ok = false;
-                    } else if (part > 0) {
-                        op.x = p.page_table[static_cast<size_t>(par) * p.max_pages + full];
-                        op.z = part;
-                        if (op.x >= p.num_pages || op.x < 0) op.x = -1;
-                        need = op.x >= 0;
+                    if (full + (part > 0) <= p.max_pages) {
+                        op.w = 1;
+                        if (part > 0) {
+                            op.x = p.page_table[static_cast<size_t>(par) * p.max_pages + full];
+                            op.z = part;
+                            if (op.x >= p.num_pages || op.x < 0) op.x = -1;
+                            need = op.x >= 0;
+                        }
                     }
                 }
                 if (op.w == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 1, row, j);
                 p.ops[j] = op;
+            } else if (ok) {
+                const int seq = p.seq_lens[row];
+                ok = seq >= 0;
+                const int last = static_cast<int>((static_cast<long long>(seq) + p.q_len - 1) >> p.page_log);
+                if (ok && p.q_len > 0 && last >= p.max_pages) report(p.status, MSK_ERR_CAPACITY, kWhere | 3, last, p.max_pages);
+                if (ok && p.q_len > 0)
+                    for (int lp = seq >> p.page_log; lp <= min(last, p.max_pages - 1); ++lp)
+                        need += p.page_table[static_cast<size_t>(row) * p.max_pages + lp] < 0;
+            } else {
+                report(p.status, MSK_ERR_BOUNDS, kWhere | 2, row, j);
             }
-            need = __shfl_sync(0xffffffffu, need, 0);
-        } else {
+            p.need[j] = ok ? need : (kFork ? 0 : -1);  // extend: -1 = refused
+        }
+    } else {
+        for (int j = gwarp; j < p.n; j += kAllWarps) {
+            const int row = p.list[j];
+            bool ok = row >= 0 && row < p.rows && __ldcg(p.claim + row) == j;
+            int need = 0;
             if (!ok && lane == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 2, row, j);
             if (ok) {
                 int seq, n_tok, first_loc;
@@ -202,15 +237,17 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
                 const int first = seq >> p.page_log;
                 const int last = n_tok > 0 ? static_cast<int>((static_cast<long long>(seq) + n_tok - 1) >> p.page_log) : first - 1;
                 if (ok && last >= p.max_pages && lane == 0) report(p.status, MSK_ERR_CAPACITY, kWhere | 3, last, p.max_pages);
-                for (int lp = first + lane; __any_sync(0xffffffffu, ok && lp <= min(last, p.max_pages - 1)); lp += 32) {
-                    const bool want = ok && lp <= min(last, p.max_pages - 1) && p.page_table[static_cast<size_t>(row) * p.max_pages + lp] < 0;
+                const int end = ok ? min(last, p.max_pages - 1) : first - 1;
+                for (int lp0 = first; lp0 <= end; lp0 += 32) {
+                    const int lp = lp0 + lane;
+                    const bool want = lp <= end && p.page_table[static_cast<size_t>(row) * p.max_pages + lp] < 0;
                     need += __popc(__ballot_sync(0xffffffffu, want));
                 }
             }
+            if (lane == 0) p.need[j] = ok ? need : -1;
         }
-        if (lane == 0) p.need[j] = ok ? need : (kFork ? 0 : -1);  // extend: -1 = refused
     }
-    cluster_exchange();
+    exchange(nct);
     // offsets of the entries (every CTA scans the whole list and keeps those its warps will serve), and the free list
     int total_need = 0;
     for (int j0 = 0; j0 < p.n; j0 += kPlanThreads) {
@@ -218,19 +255,18 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
         const int v = j < p.n ? max(__ldcg(p.need + j), 0) : 0;
         int total;
         const int before = block_scan(v, &total);
-        if (j < p.n && (j % kAllWarps) / kPlanWarps == rank) p.offs[j] = total_need + before;
+        if (j < p.n && (few ? j % kAll / kPlanThreads : j % kAllWarps / kPlanWarps) == rank) p.offs[j] = total_need + before;
         total_need += total;
     }
     int before;
-    const int total_free = slice_total(p.counts, rank, &before);
-    if (total_need > 0 && before < total_need) {
+    const int total_free = slice_total(p.counts, gwarp, kAllWarps, &before);
+    if (total_need > 0 && before < total_need && mine > 0) {
         int at = before;
         walk_refs(p.refs, lo, hi, [&](int i, const int (&r)[4], int k) {
             int c = 0;
             for (int j = 0; j < 4; ++j) c += j < k && r[j] == 0;
-            int total;
-            int w = at + block_scan(c, &total);
-            at += total;
+            int w = at + lanes_before(c);
+            at += warp_total(c);
             for (int j = 0; j < 4; ++j)
                 if (j < k && r[j] == 0) {
                     if (w < total_need) p.free_list[w] = i + j;
@@ -239,49 +275,80 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
         });
     }
     if (gtid == 0 && total_need > total_free) report(p.status, MSK_ERR_CAPACITY, kWhere | 4, total_need, total_free);
-    cluster_exchange();
-    for (int j = gwarp; j < p.n; j += kAllWarps) {
-        const int need = __ldcg(p.need + j), off = __ldcg(p.offs + j);
-        if (kFork) {
-            if (lane == 0 && need > 0) {
+    exchange(nct);
+    if (few) {
+        for (int j = gtid; j < p.n; j += kAll) {
+            const int need = __ldcg(p.need + j), off = __ldcg(p.offs + j);
+            if (need <= 0) continue;
+            if (kFork) {
                 const bool got = off < total_free;
                 const int page = got ? __ldcg(p.free_list + off) : -1;
                 p.ops[j].y = page;
                 if (got) p.refs[page] = 1;
                 else p.ops[j].w = 2;
-            }
-            continue;
-        }
-        const int row = p.list[j];
-        int seq = 0, n_tok = 0, first_loc = 0;
-        if (row >= 0 && row < p.rows) span_of(p, row, j, &seq, &n_tok, &first_loc);
-        else if (p.cu == nullptr) first_loc = j * p.q_len, n_tok = p.q_len;
-        else first_loc = min(max(p.cu[j], 0), p.tokens), n_tok = max(min(max(p.cu[j + 1], 0), p.tokens) - first_loc, 0);
-        int* held = need >= 0 ? p.page_table + static_cast<size_t>(row) * p.max_pages : nullptr;
-        if (need > 0) {
-            const int first = seq >> p.page_log;
-            const int last = min(static_cast<int>((static_cast<long long>(seq) + n_tok - 1) >> p.page_log), p.max_pages - 1);
-            int at = off;
-            for (int lp0 = first; lp0 <= last; lp0 += 32) {
-                const int lp = lp0 + lane;
-                const bool want = lp <= last && held[lp] < 0;
-                const uint32_t all = __ballot_sync(0xffffffffu, want);
-                const int k = at + __popc(all & ((1u << lane) - 1u));
-                if (want && k < total_free) {
-                    const int page = __ldcg(p.free_list + k);
-                    held[lp] = page;
-                    p.refs[page] = 1;
+            } else {
+                const int row = p.list[j], seq = p.seq_lens[row];
+                int* held = p.page_table + static_cast<size_t>(row) * p.max_pages;
+                const int last = min(static_cast<int>((static_cast<long long>(seq) + p.q_len - 1) >> p.page_log), p.max_pages - 1);
+                int k = off;
+                for (int lp = seq >> p.page_log; lp <= last; ++lp) {
+                    if (held[lp] >= 0) continue;
+                    if (k < total_free) {
+                        const int page = __ldcg(p.free_list + k);
+                        held[lp] = page;
+                        p.refs[page] = 1;
+                    }
+                    ++k;
                 }
-                at += __popc(all);
             }
-            __syncwarp();
         }
-        if (p.cache_loc != nullptr) {
-            for (int t = lane; t < n_tok; t += 32) {
-                const long long pos = static_cast<long long>(seq) + t;
-                const int page = held != nullptr && (pos >> p.page_log) < p.max_pages ? held[pos >> p.page_log] : -1;
-                p.cache_loc[static_cast<long long>(first_loc) + t] =
-                    page >= 0 ? (static_cast<long long>(page) << p.page_log) + (pos & (p.page_size - 1)) : -1;
+        if (kFork || p.cache_loc == nullptr) return;
+        exchange(nct);
+        for (int t = gtid; t < p.tokens; t += kAll) {  // a thread per token
+            const int j = t / p.q_len, row = p.list[j];
+            long long loc = -1;
+            if (__ldcg(p.need + j) >= 0) {
+                const long long pos = static_cast<long long>(p.seq_lens[row]) + (t - j * p.q_len), lp = pos >> p.page_log;
+                const int page = lp < p.max_pages ? __ldcg(p.page_table + static_cast<size_t>(row) * p.max_pages + lp) : -1;
+                if (page >= 0) loc = (static_cast<long long>(page) << p.page_log) + (pos & (p.page_size - 1));
+            }
+            p.cache_loc[t] = loc;
+        }
+        return;
+    }
+    if constexpr (!kFork) {
+        for (int j = gwarp; j < p.n; j += kAllWarps) {
+            const int need = __ldcg(p.need + j), off = __ldcg(p.offs + j), row = p.list[j];
+            int seq = 0, n_tok = 0, first_loc = 0;
+            if (row >= 0 && row < p.rows) span_of(p, row, j, &seq, &n_tok, &first_loc);
+            else if (p.cu == nullptr) first_loc = j * p.q_len, n_tok = p.q_len;
+            else first_loc = min(max(p.cu[j], 0), p.tokens), n_tok = max(min(max(p.cu[j + 1], 0), p.tokens) - first_loc, 0);
+            int* held = need >= 0 ? p.page_table + static_cast<size_t>(row) * p.max_pages : nullptr;
+            if (need > 0) {
+                const int first = seq >> p.page_log;
+                const int last = min(static_cast<int>((static_cast<long long>(seq) + n_tok - 1) >> p.page_log), p.max_pages - 1);
+                int at = off;
+                for (int lp0 = first; lp0 <= last; lp0 += 32) {
+                    const int lp = lp0 + lane;
+                    const bool want = lp <= last && held[lp] < 0;
+                    const uint32_t all = __ballot_sync(0xffffffffu, want);
+                    const int k = at + __popc(all & ((1u << lane) - 1u));
+                    if (want && k < total_free) {
+                        const int page = __ldcg(p.free_list + k);
+                        held[lp] = page;
+                        p.refs[page] = 1;
+                    }
+                    at += __popc(all);
+                }
+                __syncwarp();
+            }
+            if (p.cache_loc != nullptr) {
+                for (int t = lane; t < n_tok; t += 32) {
+                    const long long pos = static_cast<long long>(seq) + t;
+                    const int page = held != nullptr && (pos >> p.page_log) < p.max_pages ? held[pos >> p.page_log] : -1;
+                    p.cache_loc[static_cast<long long>(first_loc) + t] =
+                        page >= 0 ? (static_cast<long long>(page) << p.page_log) + (pos & (p.page_size - 1)) : -1;
+                }
             }
         }
     }
@@ -367,24 +434,25 @@ __global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(PlanArgs p, Ca
     }
 }
 
-// Compact, first launch (one cluster): with n pages in use, the k-th page in use from n on goes to the k-th free page below n.
-__global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1) pages_compact_plan_kernel(PlanArgs p) {
-    const int tid = threadIdx.x;
-    const int rank = static_cast<int>(cluster_ctarank());
-    const int gtid = rank * kPlanThreads + tid;
-    constexpr int kAll = kCluster * kPlanThreads;
+// Compact, first launch: with n pages in use, the k-th page in use from n on goes to the k-th free page below n.
+__global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(PlanArgs p) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = blockIdx.x, nct = gridDim.x;
+    const int gtid = rank * kPlanThreads + tid, gwarp = rank * kPlanWarps + warp;
+    const int kAll = nct * kPlanThreads, kAllWarps = nct * kPlanWarps;
+    int *c_live = p.counts, *c_hole = c_live + kCluster * kPlanWarps, *c_move = c_hole + kCluster * kPlanWarps, *result = c_move + kCluster * kPlanWarps;
     pdl_wait();
     pdl_launch_dependents();
     int lo, hi;
-    slice_of(p, rank, &lo, &hi);
-    int mine = 0, total, before;
+    slice_of(p, gwarp, kAllWarps, &lo, &hi);
+    int mine = 0, before;
     walk_refs(p.refs, lo, hi, [&](int, const int (&r)[4], int k) {
         for (int j = 0; j < 4; ++j) mine += j < k && r[j] > 0;
     });
-    block_scan(mine, &total);
-    if (tid == 0) p.counts[rank] = total;
-    cluster_exchange();
-    const int live = slice_total(p.counts, rank, &before);
+    mine = warp_total(mine);
+    if (lane == 0) c_live[gwarp] = mine;
+    exchange(nct);
+    const int live = slice_total(c_live, gwarp, kAllWarps, &before);
     // a page below `live` that is free, or one in use from `live` on: as many of the one as of the other
     auto kind = [&](int page, int r) { return page < live ? (r <= 0 ? 1 : 0) : (r > 0 ? 2 : 0); };
     int holes = 0, moves = 0;
@@ -394,30 +462,30 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
             holes += t == 1, moves += t == 2;
         }
     });
-    block_scan(holes, &total);
-    if (tid == 0) p.counts[kCluster + rank] = total;
-    block_scan(moves, &total);
-    if (tid == 0) p.counts[2 * kCluster + rank] = total;
-    cluster_exchange();
+    holes = warp_total(holes), moves = warp_total(moves);
+    if (lane == 0) c_hole[gwarp] = holes, c_move[gwarp] = moves;
+    exchange(nct);
     int hole_at, move_at;
-    slice_total(p.counts + kCluster, rank, &hole_at);
-    const int all_moves = slice_total(p.counts + 2 * kCluster, rank, &move_at);
-    walk_refs(p.refs, lo, hi, [&](int i, const int (&r)[4], int k) {
-        int nh = 0, nm = 0;
-        for (int j = 0; j < 4; ++j) {
-            const int t = j < k ? kind(i + j, r[j]) : 0;
-            nh += t == 1, nm += t == 2;
-        }
-        int th, tm;
-        int wh = hole_at + block_scan(nh, &th), wm = move_at + block_scan(nm, &tm);
-        hole_at += th, move_at += tm;
-        for (int j = 0; j < 4; ++j) {
-            const int t = j < k ? kind(i + j, r[j]) : 0;
-            if (t == 1) p.dst[wh++] = i + j;
-            if (t == 2) p.src[wm++] = i + j;
-        }
-    });
-    cluster_exchange();
+    slice_total(c_hole, gwarp, kAllWarps, &hole_at);
+    const int all_moves = slice_total(c_move, gwarp, kAllWarps, &move_at);
+    if (holes + moves > 0) {
+        walk_refs(p.refs, lo, hi, [&](int i, const int (&r)[4], int k) {
+            int nh = 0, nm = 0;
+            for (int j = 0; j < 4; ++j) {
+                const int t = j < k ? kind(i + j, r[j]) : 0;
+                nh += t == 1, nm += t == 2;
+            }
+            const int both = lanes_before(nh | nm << 16);  // at most 128 of either in a step
+            int wh = hole_at + (both & 0xffff), wm = move_at + (both >> 16);
+            hole_at += warp_total(nh), move_at += warp_total(nm);
+            for (int j = 0; j < 4; ++j) {
+                const int t = j < k ? kind(i + j, r[j]) : 0;
+                if (t == 1) p.dst[wh++] = i + j;
+                if (t == 2) p.src[wm++] = i + j;
+            }
+        });
+    }
+    exchange(nct);
     for (int k = gtid; k < all_moves; k += kAll) {
         const int s = __ldcg(p.src + k), d = __ldcg(p.dst + k);
         p.remap[s] = d;
@@ -425,7 +493,7 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
         p.refs[s] = 0;
     }
     if (gtid == 0) {
-        p.counts[3 * kCluster] = live, p.counts[3 * kCluster + 1] = all_moves;
+        result[0] = live, result[1] = all_moves;
         if (p.result != nullptr) p.result[0] = live, p.result[1] = all_moves;
     }
 }
@@ -434,7 +502,8 @@ __global__ void __launch_bounds__(kPlanThreads) __cluster_dims__(kCluster, 1, 1)
 __global__ void __launch_bounds__(kCopyThreads) pages_compact_kernel(PlanArgs p, Caches caches) {
     pdl_wait();
     pdl_launch_dependents();
-    const int live = __ldcg(p.counts + 3 * kCluster), moves = __ldcg(p.counts + 3 * kCluster + 1);
+    const int* result = p.counts + 3 * kCluster * kPlanWarps;
+    const int live = __ldcg(result), moves = __ldcg(result + 1);
     if (moves == 0) return;
     const long long entries = static_cast<long long>(p.rows) * p.max_pages;
     for (long long i = static_cast<long long>(blockIdx.x) * kCopyThreads + threadIdx.x; i < entries; i += static_cast<long long>(gridDim.x) * kCopyThreads) {
@@ -463,7 +532,7 @@ size_t layout(const MskPages* q, int n, uint8_t* ws, PlanArgs* a) {
         at += up256(bytes);
         return p;
     };
-    int* counts = reinterpret_cast<int*>(take((3 * kCluster + 4) * 4));
+    int* counts = reinterpret_cast<int*>(take((3 * kCluster * kPlanWarps + 4) * 4));
     int* claim = reinterpret_cast<int*>(take(static_cast<size_t>(q->rows) * 4));
     int* is_parent = reinterpret_cast<int*>(take(static_cast<size_t>(q->rows) * 4));
     int* need = reinterpret_cast<int*>(take(static_cast<size_t>(n) * 4));
@@ -508,14 +577,29 @@ int fill_caches(const MskPages* q, void* const* caches, int n_caches, int token_
 }
 
 template <class... Params, class... Args>
-int launch(void (*kernel)(Params...), unsigned grid, unsigned block, bool chained, void* stream, Args... args) {
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+int launch(void (*kernel)(Params...), unsigned grid, unsigned block, bool chained, unsigned cluster, void* stream, Args... args) {
+    cudaLaunchAttribute attr[2];
+    int n = 0;
     cudaLaunchConfig_t cfg = {};
+    if (chained) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
     cfg.gridDim = dim3(grid), cfg.blockDim = dim3(block), cfg.stream = static_cast<cudaStream_t>(stream);
-    cfg.attrs = &attr, cfg.numAttrs = chained ? 1 : 0;
+    cfg.attrs = attr, cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : MSK_ERR_CUDA;
+}
+
+// A planning kernel: one CTA, or one cluster of eight where there is much to rank or to look up.
+template <class... Params>
+int launch_plan(void (*kernel)(Params...), const PlanArgs& a, void* stream) {
+    const unsigned n = a.num_pages > kOneCta || a.n > 1024 ? kCluster : 1;
+    return launch(kernel, n, kPlanThreads, false, n, stream, a);
 }
 
 // CTAs for page data: enough to fill every SM, no more than there are pieces.
@@ -530,7 +614,7 @@ int drop(const MskPages* q, const int* rows, int n, int window, int sinks, int t
     if (rc != 0 || n == 0) return rc;
     const int per_row = (q->max_pages + 1023) / 1024;
     if (static_cast<long long>(n) * per_row > 0x7fffffffll) return MSK_ERR_UNSUPPORTED;
-    return launch(pages_drop_kernel, static_cast<unsigned>(n) * per_row, 256, false, stream, a, per_row, window, sinks, trim);
+    return launch(pages_drop_kernel, static_cast<unsigned>(n) * per_row, 256, false, 1, stream, a, per_row, window, sinks, trim);
 }
 
 }  // namespace
@@ -563,7 +647,7 @@ extern "C" int msk_pages_extend(const MskPages* q, const int32_t* rows, int n, i
     if (n == 0) return 0;
     a.q_len = q_len, a.cu = cu_seqlens, a.tokens = cu_seqlens != nullptr ? tokens : n * q_len;
     a.cache_loc = reinterpret_cast<long long*>(cache_loc);
-    return launch(pages_plan_kernel<false>, kCluster, kPlanThreads, false, stream, a);
+    return launch_plan(pages_plan_kernel<false>, a, stream);
 }
 
 extern "C" int msk_pages_fork(const MskPages* q, const int32_t* parents, const int32_t* children, int n, void* const* caches, int n_caches,
@@ -582,9 +666,9 @@ extern "C" int msk_pages_fork(const MskPages* q, const int32_t* parents, const i
     const long long chunks = (static_cast<long long>(q->page_size) * token_bytes + kCopyChunk - 1) / kCopyChunk;
     const unsigned data = copy_ctas(static_cast<long long>(n) * n_caches * chunks);
     if (row_blocks + data > 0x7fffffffll) return MSK_ERR_UNSUPPORTED;
-    rc = launch(pages_plan_kernel<true>, kCluster, kPlanThreads, false, stream, a);
+    rc = launch_plan(pages_plan_kernel<true>, a, stream);
     if (rc != 0) return rc;
-    return launch(pages_fork_kernel, static_cast<unsigned>(row_blocks) + data, kCopyThreads, true, stream, a, c, static_cast<int>(row_blocks), per_row);
+    return launch(pages_fork_kernel, static_cast<unsigned>(row_blocks) + data, kCopyThreads, true, 1, stream, a, c, static_cast<int>(row_blocks), per_row);
 }
 
 extern "C" int msk_pages_compact(const MskPages* q, void* const* caches, int n_caches, int token_bytes, int32_t* result, void* scratch,
@@ -597,10 +681,10 @@ extern "C" int msk_pages_compact(const MskPages* q, void* const* caches, int n_c
     rc = fill_caches(q, caches, n_caches, token_bytes, &c);
     if (rc != 0) return rc;
     a.result = result;
-    rc = launch(pages_compact_plan_kernel, kCluster, kPlanThreads, false, stream, a);
+    rc = launch_plan(pages_compact_plan_kernel, a, stream);
     if (rc != 0) return rc;
     const long long chunks = (static_cast<long long>(q->page_size) * token_bytes + kCopyChunk - 1) / kCopyChunk;
     const long long table = (static_cast<long long>(q->rows) * q->max_pages + kCopyThreads - 1) / kCopyThreads;
     const long long data = static_cast<long long>(q->num_pages / 2 + 1) * n_caches * chunks;  // at most half of the pages move
-    return launch(pages_compact_kernel, copy_ctas(data > table ? data : table), kCopyThreads, true, stream, a, c);
+    return launch(pages_compact_kernel, copy_ctas(data > table ? data : table), kCopyThreads, true, 1, stream, a, c);
 }
