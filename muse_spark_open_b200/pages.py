@@ -12,7 +12,8 @@ that uses the pool.  A step of a serving loop:
     pool["seq_lens"][rows] += q_len                       # the tokens that stay (fewer after a rejected draft)
     pages.trim(pool, rows, window, sinks)                 # what the window has passed goes back
 
-Everything happens on the device, in place and in stream order; nothing is read back, so all calls can be captured in a CUDA
+Everything happens on the device, in place and in stream order (order the streams yourself when you use several on one pool);
+nothing is read back, so all calls can be captured in a CUDA
 graph.  New pages are the lowest free ones, given out in the order of the rows: results do not depend on scheduling.
 Problems with the contents (a row out of range or listed twice, no free page) are reported in the status word
 (`abi.status_for(device).raise_if_set()`), and the entries concerned are skipped; include/msk.h says how.
@@ -38,7 +39,6 @@ def prepare(num_pages: int, page_size: int, rows: int, max_pages: int, device="c
 
 _pages_args = abi.packer(abi.Pages)
 _INT = torch.int32
-_bytes: dict = {}
 
 
 def _args(pool: dict, *lists: torch.Tensor):
@@ -56,18 +56,19 @@ def _args(pool: dict, *lists: torch.Tensor):
     return _pages_args.pack(table.data_ptr(), seq.data_ptr(), refs.data_ptr(), rows, most, pages, pool["page_size"]), (rows, pages), index
 
 
-def _scratch(q: bytes, shape, n: int, like: torch.Tensor):
-    # the size is a function of sizes alone; the memory comes from torch's allocator, on the current stream: calls on other
-    # streams and other captured graphs get other memory
-    key = (*shape, n)
-    size = _bytes.get(key)
-    if size is None:
-        b = C.c_size_t()
-        abi.check(abi.lib().msk_pages_scratch_bytes(q, n, C.byref(b)), "msk_pages_scratch_bytes")
-        if len(_bytes) > 4096:
-            _bytes.clear()
-        size = _bytes[key] = b.value
-    return torch.empty(size, dtype=torch.uint8, device=like.device), size
+def _scratch(pool: dict, q: bytes, shape, n: int):
+    """(address, bytes) of the pool's workspace, kept in the pool from its first call on: calls on one pool change the same
+    counts and are ordered anyway.  Lists longer than the pool has rows (and a first call inside a graph capture, whose memory
+    is the graph's) get memory of their own, for the call."""
+    kept = pool.get("scratch")
+    if kept is not None and kept[0] == shape and n <= shape[0]:
+        return kept[1], kept[2], None
+    b = C.c_size_t()
+    abi.check(abi.lib().msk_pages_scratch_bytes(q, max(n, shape[0]), C.byref(b)), "msk_pages_scratch_bytes")
+    t = torch.empty(b.value, dtype=torch.uint8, device=pool["refs"].device)
+    if kept is None and n <= shape[0] and not torch.cuda.is_current_stream_capturing():
+        pool["scratch"] = (shape, t.data_ptr(), b.value, t)
+    return t.data_ptr(), b.value, t
 
 
 def _caches(caches, pool: dict, index: int):
@@ -100,8 +101,8 @@ def extend(pool: dict, rows: torch.Tensor, q_len: int = 1, cu_seqlens: torch.Ten
         if cu_seqlens.shape[0] != n + 1:
             raise abi.MskError("cu_seqlens must have one entry more than rows")
         loc, cu = torch.full((tokens,), -1, dtype=torch.int64, device=rows.device), cu_seqlens.data_ptr()
-    ws, size = _scratch(q, shape, n, rows)
-    rc = abi.lib().msk_pages_extend(q, rows.data_ptr(), n, q_len, cu, tokens, loc.data_ptr(), ws.data_ptr(), size, abi.status_ptr(index),
+    ws, size, _own = _scratch(pool, q, shape, n)
+    rc = abi.lib().msk_pages_extend(q, rows.data_ptr(), n, q_len, cu, tokens, loc.data_ptr(), ws, size, abi.status_ptr(index),
                                     abi.raw_stream(index))
     if rc:
         abi.check(rc, "msk_pages_extend")
@@ -117,8 +118,8 @@ def fork(pool: dict, parents: torch.Tensor, children: torch.Tensor, caches) -> N
     if parents.shape[0] != n:
         raise abi.MskError("parents and children must have the same length")
     ptrs, count, token = _caches(caches, pool, index)
-    ws, size = _scratch(q, shape, n, children)
-    rc = abi.lib().msk_pages_fork(q, parents.data_ptr(), children.data_ptr(), n, ptrs, count, token, ws.data_ptr(), size, abi.status_ptr(index),
+    ws, size, _own = _scratch(pool, q, shape, n)
+    rc = abi.lib().msk_pages_fork(q, parents.data_ptr(), children.data_ptr(), n, ptrs, count, token, ws, size, abi.status_ptr(index),
                                   abi.raw_stream(index))
     if rc:
         abi.check(rc, "msk_pages_fork")
@@ -145,10 +146,9 @@ def compact(pool: dict, caches) -> torch.Tensor:
     follows.  Returns int32 [2] on the device: n, and how many pages moved."""
     q, shape, index = _args(pool)
     ptrs, count, token = _caches(caches, pool, index)
-    refs = pool["refs"]
-    ws, size = _scratch(q, shape, 0, refs)
-    result = torch.empty(2, dtype=_INT, device=refs.device)
-    rc = abi.lib().msk_pages_compact(q, ptrs, count, token, result.data_ptr(), ws.data_ptr(), size, abi.status_ptr(index), abi.raw_stream(index))
+    ws, size, _own = _scratch(pool, q, shape, 0)
+    result = torch.empty(2, dtype=_INT, device=pool["refs"].device)
+    rc = abi.lib().msk_pages_compact(q, ptrs, count, token, result.data_ptr(), ws, size, abi.status_ptr(index), abi.raw_stream(index))
     if rc:
         abi.check(rc, "msk_pages_compact")
     return result

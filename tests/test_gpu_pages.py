@@ -165,6 +165,21 @@ def test_calls_in_a_graph_and_on_another_stream():
     assert not status()
 
 
+def test_lists_longer_than_the_pool_and_the_kept_workspace():
+    """More list entries than rows (all but the first of a row are refused), before and after the workspace is kept."""
+    from muse_spark_open_b200 import pages
+    model = Pool(64, 16, 4, 8)
+    pool, _, _ = upload(model, [])
+    for listed in ([0, 1, 0, 2, 3, 3, 1, 0, 2], [2, 0], [3, 2, 1, 0, 0, 1, 2, 3]):
+        loc = pages.extend(pool, i32(listed), 20)
+        want, bad = model.extend(listed, [20] * len(listed))
+        assert loc.tolist() == want and status() == bad
+        same(model, pool)
+    first = pool["scratch"][1]
+    pages.compact(pool, [])
+    assert pool["scratch"][1] == first and not status()
+
+
 def test_nothing_to_do():
     from muse_spark_open_b200 import pages
     pool = pages.prepare(8, 16, 4, 4)
