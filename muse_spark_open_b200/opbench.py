@@ -2,7 +2,9 @@
 bench.py files, e.g. muse_moe_w4a16/bench.py): cold-L2 device time, achieved GB/s over algorithmic bytes.
 
     python -m muse_spark_open_b200.opbench proj  [--m 16 --n 6144 --k 4096 --splits 0]
-    python -m muse_spark_open_b200.opbench attn  [--batch 16 --ctx 1024:8192 --window 1024 --q-len 1]
+    python -m muse_spark_open_b200.opbench attn  [--batch 16 --ctx 1024:8192 --window 1024 --sinks 0 --q-len 1]
+    python -m muse_spark_open_b200.opbench prompt [--new 8192 --batch 16 --ctx 1024:8192 --window 1024 --sinks 0]
+    python -m muse_spark_open_b200.opbench pages [--batch 16 --ctx 1024:8192 --window 1024 --sinks 0]
     python -m muse_spark_open_b200.opbench moe   [--tokens 32]
     python -m muse_spark_open_b200.opbench layer [--batch 32 --ctx 8192 --q-len 1]
 
@@ -16,7 +18,7 @@ import json
 
 import torch
 
-from . import abi, attention, layer, moe, proj, synth, timing
+from . import abi, attention, layer, moe, pages, proj, synth, timing
 
 DEV = "cuda"
 
@@ -58,15 +60,57 @@ def run_attn(a):
     seqs = _seqs(a, a.batch)
     data = synth.make_layer_input(0, DEV, seqs, q_len=a.q_len, window=a.window, rope_theta=1e6 if a.window else 0.0)
     cfg = data["config"]
+    cfg["sinks"] = a.sinks
     t = a.batch * a.q_len
     g = torch.Generator(device=DEV).manual_seed(2)
     qkv = torch.randn((t, 9216), generator=g, device=DEV).to(torch.bfloat16)
     out = torch.empty((t, 4096), dtype=torch.bfloat16, device=DEV)
     us = _time(lambda: attention.launch(qkv, out, data, cfg, chunks=a.chunks, stages=a.stages, issuers=a.issuers,
                                          row_groups=a.row_groups), a)
-    keys = sum(min(s, a.window - 1) if a.window else s for s in seqs)
+    keys = sum(min(s, a.window - 1 + min(a.sinks, max(0, s - a.window + 1))) if a.window else s for s in seqs)
     _emit("attn_decode", us, keys * 4 * 128 * 2 + t * (9216 + 4096) * 2, batch=a.batch, q_len=a.q_len, window=a.window,
           ctx=a.ctx, chunks=a.chunks, stages=a.stages, issuers=a.issuers)
+
+
+def run_prompt(a):
+    """Prompts of --new tokens each behind --ctx cached ones: prep + attention (+ combine)."""
+    seqs, n = _seqs(a, a.batch), a.new
+    data = synth.make_layer_input(0, DEV, seqs, q_len=n, window=a.window, rope_theta=1e6)
+    cfg = dict(data["config"], sinks=a.sinks)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    data.update(qkv=torch.randn((a.batch * n, 9216), generator=g, device=DEV).to(torch.bfloat16), config=cfg,
+                cu_seqlens_q=torch.arange(0, a.batch * n + 1, n, dtype=torch.int32, device=DEV))
+    out = torch.empty((a.batch * n, 4096), dtype=torch.bfloat16, device=DEV)
+    us = _time(lambda: attention.prompt_fn(data, out=out), a)
+    pairs = sum(sum(min(t + 1, a.window + min(a.sinks, max(0, t + 1 - a.window))) if a.window else t + 1 for t in range(s, s + n)) for s in seqs)
+    flops = 4 * 128 * 32 * pairs
+    extra = {} if us is None else {"tflops": round(flops / us / 1e6, 1)}
+    _emit("attn_prompt", us, a.batch * n * (9216 + 4096) * 2 + sum(s + n for s in seqs) * 4 * 128 * 2, batch=a.batch, new=n, ctx=a.ctx, window=a.window,
+          sinks=a.sinks, **extra)
+
+
+def run_pages(a):
+    """A full pool: half of the requests leave, the others give back what their window has passed, the rest moves to the front."""
+    seqs = _seqs(a, a.batch)
+    data = synth.make_layer_input(0, DEV, seqs, q_len=1, window=a.window)
+    table, caches = data["page_table"], [data["k_cache"], data["v_cache"]]
+    refs = torch.zeros(caches[0].shape[0], dtype=torch.int32, device=DEV)
+    refs[table[table >= 0].long()] = 1
+    pool = {"page_table": table, "seq_lens": data["seq_lens"], "refs": refs, "page_size": 64}
+    was = {k: pool[k].clone() for k in ("page_table", "seq_lens", "refs")}
+    rows = torch.arange(a.batch, dtype=torch.int32, device=DEV)
+    moved = []
+
+    def fn():
+        for k, v in was.items():
+            pool[k].copy_(v)
+        pages.free(pool, rows[a.batch // 2:])
+        pages.trim(pool, rows[:a.batch // 2], a.window, a.sinks)
+        moved[:] = [pages.compact(pool, caches)]
+    fn()
+    n = int(moved[0][1])
+    us = _time(fn, a)
+    _emit("pages free + trim + compact", us, 2 * n * 2 * 64 * 4 * 128, batch=a.batch, ctx=a.ctx, window=a.window, sinks=a.sinks, moved=n)
 
 
 def run_moe(a):
@@ -104,7 +148,7 @@ def run_layer(a):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("op", choices=["proj", "attn", "moe", "layer"])
+    ap.add_argument("op", choices=["proj", "attn", "prompt", "pages", "moe", "layer"])
     ap.add_argument("--m", type=int, default=16)
     ap.add_argument("--n", type=int, default=6144)
     ap.add_argument("--k", type=int, default=4096)
@@ -112,6 +156,8 @@ def main():
     ap.add_argument("--batch", type=int, default=16)
     ap.add_argument("--ctx", default="1024:8192")
     ap.add_argument("--window", type=int, default=1024)
+    ap.add_argument("--sinks", type=int, default=0)
+    ap.add_argument("--new", type=int, default=8192)
     ap.add_argument("--q-len", type=int, default=1)
     ap.add_argument("--chunks", type=int, default=0)
     ap.add_argument("--stages", type=int, default=0)
@@ -124,7 +170,7 @@ def main():
     ap.add_argument("--reps", type=int, default=10)
     ap.add_argument("--eager", type=int, default=0)
     a = ap.parse_args()
-    {"proj": run_proj, "attn": run_attn, "moe": run_moe, "layer": run_layer}[a.op](a)
+    {"proj": run_proj, "attn": run_attn, "prompt": run_prompt, "pages": run_pages, "moe": run_moe, "layer": run_layer}[a.op](a)
     abi.status_for(DEV).raise_if_set(a.op)
 
 
