@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     const int W = p.window;
     // The tiles with visible keys: those of the first `sinks` positions that lie wholly before the window's first tile,
     // then the window's.  The chunks of the cluster split this list; `gap` tiles between the two parts are skipped.
-    const int snk = W > 0 ? p.sinks : 0;
+    const int snk = p.sinks;  // 0 without a window
     const int lo_all = W > 0 ? max(0, seq - W + 1) : 0;
     const int t_first = lo_all / kTileKeys;
     const int sink_tiles = min((min(snk, seq) + kTileKeys - 1) / kTileKeys, t_first);
@@ -791,10 +791,11 @@ template <int L, int RG>
 int launch_attn(const MskAttnParams* q, int* status, cudaStream_t stream) {
     constexpr int NR = 8 * L, NP = 2 * NR;
     constexpr int kColsHost = attn_tmem_cols(L);
+    const int sinks = q->window > 0 ? q->sinks : 0;
     const int tile_cap = (q->max_pages * q->page_size + kTileKeys - 1) / kTileKeys;
     int tiles_max = tile_cap;
     if (q->window > 0)  // the window's tiles and the sinks', each at an unknown offset
-        tiles_max = min(static_cast<long long>(tiles_max), static_cast<long long>(q->window / kTileKeys) + q->sinks / kTileKeys + 2 + (q->sinks > 0 ? 1 : 0));
+        tiles_max = min(static_cast<long long>(tiles_max), static_cast<long long>(q->window / kTileKeys) + 2 + (sinks > 0 ? sinks / kTileKeys + 1 : 0));
     if (tiles_max < 1) tiles_max = 1;
     // the ring needs 3 slots: a tile's slot is refilled one iteration after its tile (finish_tile runs late),
     // and the next tile's scores are issued one iteration early
@@ -813,7 +814,7 @@ int launch_attn(const MskAttnParams* q, int* status, cudaStream_t stream) {
         // more (request, head) pairs than CTA slots but fewer than two waves of them, and long contexts: halves
         // balance the last wave better; with several waves (longest first) whole contexts have less fixed cost
         // (under a window with sinks the contexts are alike: 64 requests x 4 heads, window 4096: 56 us in one chunk, 67 in two)
-        if (C == 1 && tiles_max >= 32 && q->B * q->Hkv < 2 * resident * 148 && !(q->window > 0 && q->sinks > 0)) C = 2;
+        if (C == 1 && tiles_max >= 32 && q->B * q->Hkv < 2 * resident * 148 && sinks == 0) C = 2;
         while ((tiles_max + C - 1) / C > kMaxTilesPerCta && C < 8) C *= 2;
     }
     if (C != 1 && C != 2 && C != 4 && C != 8) return MSK_ERR_INVALID;
@@ -851,7 +852,7 @@ int launch_attn(const MskAttnParams* q, int* status, cudaStream_t stream) {
         a.longest_first = 1;
         while (a.longest_first < (1 << 29) && 2ll * a.longest_first <= most) a.longest_first *= 2;
     }
-    a.window = q->window, a.sinks = q->sinks, a.nstages = nst, a.qk_scale_factor = q->qk_scale_factor, a.sm_scale = q->sm_scale;
+    a.window = q->window, a.sinks = sinks, a.nstages = nst, a.qk_scale_factor = q->qk_scale_factor, a.sm_scale = q->sm_scale;
     // largest power of two that keeps |q| * scale <= 448 (|q| <= qk_scale_factor * sqrt(128) after RMSNorm)
     float qs = 1.0f;
     const float qmax = fabsf(q->qk_scale_factor) * 11.3137085f;
