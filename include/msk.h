@@ -125,7 +125,7 @@ int msk_attn_decode(const MskAttnParams* p, int* status, void* stream);
  * cu_seqlens_q[b+1]) of qkv, its new tokens at positions seq_lens[b], seq_lens[b] + 1, ...; their keys and values are
  * quantised and written into the pages the page table names for those positions, and attended from there.  Tokens see the
  * positions up to their own inside the window, and the first `sinks` ones.  Requests may bring no token; rows of qkv / out
- * outside every request are neither read nor written.  A new token whose position has no page (-1, or beyond max_pages)
+ * outside every request do not matter and stay as they are.  A new token whose position has no page (-1, or beyond max_pages)
  * is reported in `status` and not written.  Reads of a page-table entry of -1 below the window and above the sinks never
  * happen.  Stands beside msk_attn_decode, whose counterpart in the reference has only 1 or 8 new tokens per request
  * (muse_attention_decode/submission.py:2363-2372).

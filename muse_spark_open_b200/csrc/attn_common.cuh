@@ -33,12 +33,24 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return y;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 y;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(y.x), "=f"(y.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 // 2^x for two x <= 64 on the FMA pipe (the special-function unit does 4 per clock and scheduler, which bounds a softmax of
 // wide tiles): x = n + f with n whole and |f| <= 1/2 (adding and subtracting 1.5 x 2^23 rounds to whole numbers), 2^f by
-// a polynomial of degree 3 fitted for the smallest largest relative error (7.5e-5, a third of FP16's rounding), 2^n by
-// adding n to the exponent.  Below 2^-126: 2^-126 instead of less.
+// a polynomial of degree 3 fitted for the smallest largest relative error (7.5e-5, a third of FP16's rounding), times 2^n
+// put together from its exponent.  Below 2^-126: 2^-126 instead of less.  NaN stays NaN.
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
-    x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+    x.x = max_nan(x.x, -126.0f), x.y = max_nan(x.y, -126.0f);
     const float2 big = make_float2(12582912.0f, 12582912.0f);
     const float2 t = add2(x, big);
     const float2 n = add2(t, make_float2(-12582912.0f, -12582912.0f));
@@ -46,8 +58,7 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
     float2 p = fma2(f, make_float2(0.055171702f, 0.055171702f), make_float2(0.2426112f, 0.2426112f));
     p = fma2(p, f, make_float2(0.69326097f, 0.69326097f));
     p = fma2(p, f, make_float2(0.99992806f, 0.99992806f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+    return mul2(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 __device__ __forceinline__ float redux_max(float v) {
     float r;

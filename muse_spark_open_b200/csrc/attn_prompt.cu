@@ -255,6 +255,10 @@ __global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
 __device__ __forceinline__ uint32_t low_bits(int n) {  // bits [0, n) set, n clamped to [0, 32]
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
+__device__ __forceinline__ bool has_nan(uint4 v) {  // one of 16 E4M3 values is NaN (0x7f with either sign)
+    const uint32_t k = 0x7f7f7f7fu, one = 0x01010101u;
+    return ((((v.x & k) + one) | ((v.y & k) + one) | ((v.z & k) + one) | ((v.w & k) + one)) & 0x80808080u) != 0;
+}
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
@@ -276,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[4 * SS + 4 * NS + 14];
     __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t spoilt[2];  // one bit per token of the unit: it sees a NaN value at a position others do not see
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = CG == 1 ? 0 : static_cast<int>(cluster_ctarank());  // which half of the pair; the even one issues the MMAs
@@ -307,6 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i) mbar_init(s_done + 8 * i, 1), mbar_init(p_ready + 8 * i, 4 * CG);
         mbar_init(q_here, 1);
         mbar_init(q_full, CG);
+        spoilt[0] = spoilt[1] = 0;
         fence_mbar_init();
     }
     if (tid == 64) prefetch_tmap(&tm_q), prefetch_tmap(&tm_k), prefetch_tmap(&tm_v);
@@ -452,9 +458,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) gate[e] = __ldg(src + e);
             }
-            ok = mbar_wait(o_done + 8 * g, 0, p.status, where | 4) && ok;
+            ok = mbar_wait<0, (CG > 1)>(o_done + 8 * g, 0, p.status, where | 4) && ok;
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
+            // one NaN channel makes the row's norm, and so the row, NaN
+            if (live && (*static_cast<volatile uint32_t*>(&spoilt[j >> 5]) >> (j & 31) & 1)) l = __int_as_float(0x7fffffff);
             if (p.splits == 1) {
                 const float inv = v_scale / l;
                 float ss = 0.0f;
@@ -553,12 +561,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                         in[e] = *reinterpret_cast<const uint4*>(src + rr[e] * 128 + cc[e] * 16);
                     }
                 }
-                if (kv && (s0 + kTile - 1 > p_last || (W > 0 && s0 <= p_first - W && s0 + kTile > snk))) {
-                    // values no token sees may be anything (even NaN): zeros, so that 0 * V stays 0
+                if (kv && (s0 + kTile - 1 > p_first || (W > 0 && s0 <= p_last - W && s0 + kTile > snk))) {
+                    // Positions that not all tokens of the unit see.  What none sees may be anything: zeros, so that 0 * V
+                    // stays 0.  A NaN that some see must not reach the others by 0 * V either: zeros, and a note to those.
+                    uint32_t notes = 0;
+                    auto seen = [&](int pos, int* from, int* to) {  // tokens [from, to) of the unit see position pos
+                        *from = max(pos - p_first, 0);
+                        *to = W > 0 && pos >= snk && pos - p_first < n_tok - W ? pos - p_first + W : n_tok;
+                    };
 #pragma unroll
                     for (int e = 0; e < U; ++e) {
-                        const int at = s0 + rr[e];
-                        if (at > p_last || (W > 0 && at <= p_first - W && at >= snk)) in[e] = make_uint4(0, 0, 0, 0);
+                        int from, to;
+                        seen(s0 + rr[e], &from, &to);
+                        const bool none = from >= to, bad = !none && to - from < n_tok && has_nan(in[e]);
+                        if (none || bad) in[e] = make_uint4(0, 0, 0, 0);
+                        notes |= bad ? 1u << e : 0u;
+                    }
+                    if (notes != 0) {
+#pragma unroll 1
+                        for (int e = 0; e < U; ++e) {
+                            if (!(notes >> e & 1)) continue;
+                            int from, to;
+                            seen(s0 + w * 32 + (CG == 2 ? e : e >> 1) * 8 + (lane >> 2), &from, &to);
+                            for (int c = 0; c < 2; ++c) {
+                                const uint32_t who = low_bits(to - 32 * c) & ~low_bits(from - 32 * c);
+                                atomicOr(&spoilt[c], who);
+                                if constexpr (CG == 2) dsmem_or_b32(dsmem_addr(smem_u32(&spoilt[c]), rank ^ 1), who);
+                            }
+                        }
+                        if (CG == 2) __threadfence();  // before the arrival at the even CTA, which releases at CTA scope
                     }
                 }
 #pragma unroll
@@ -732,14 +763,14 @@ __global__ void __launch_bounds__(256) prompt_combine_kernel(PromptArgs p) {
     for (int s = 0; s < p.splits; ++s) {
         const size_t r = s * stride + row;
         const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * r);
-        if (ml.y > 0.0f) {  // a split without keys has written no output
+        if (ml.y != 0.0f) {  // a split without keys has written no output; NaN counts
             const float w = ex2(ml.x - m);
             const float4 v = *reinterpret_cast<const float4*>(p.part_o + r * 128 + 4 * lane);
             l += w * ml.y;
             o[0] += w * v.x, o[1] += w * v.y, o[2] += w * v.z, o[3] += w * v.w;
         }
     }
-    const float inv = l > 0.0f ? __ldg(p.v_scale) / l : 0.0f;
+    const float inv = l != 0.0f ? __ldg(p.v_scale) / l : 0.0f;
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= inv, ss += o[i] * o[i];

@@ -125,6 +125,44 @@ def test_page_ids_and_positions_that_do_not_exist():
         abi.status_for("cuda").raise_if_set("past the table")
 
 
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("new", [40, 20])  # pairs of CTAs, and single ones
+@pytest.mark.parametrize("at", [0, 1, 5, 6, 7, 38, 70, 127, 150])
+def test_nan_in_a_visible_key_or_value_is_seen(at, new, splits):
+    """A NaN byte in the cache reaches every row that sees it, wherever it lies in the tile, and no other."""
+    from muse_spark_open_b200 import abi, attention
+    for what in ("k_cache", "v_cache"):
+        for channel in (17, 100):
+            data = make_prompt([200], [new], 3, hkv=1, window=100)
+            seen = [j for j in range(new) if 200 + j - 100 < at <= 200 + j]
+            page = int(data["page_table"][0, at // 64])
+            if page < 0:
+                continue
+            data[what].view(torch.uint8)[page, at % 64, 0, channel] = 0x7F
+            out = attention.prompt_fn(oattn.to_device(data, "cuda"), splits=splits).cpu().view(new, -1)
+            torch.cuda.synchronize()
+            abi.status_for("cuda").raise_if_set("nan")
+            bad = torch.isnan(out.float()).any(1).nonzero()[:, 0].tolist()
+            assert bad == seen, (what, at)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 0), (20, 130), (300, 4)])
+@pytest.mark.parametrize("new,at", [(150, 0), (150, 77), (150, 149), (30, 13), (30, 31 - 2)])
+def test_a_spoilt_token_spoils_no_earlier_one(new, at, window, sinks, splits):
+    """A new token with a NaN value: its own row and the later ones that see it become NaN, the others stay as they were."""
+    from muse_spark_open_b200 import abi, attention
+    data = make_prompt([90], [new], 8, hkv=1, window=window, sinks=sinks)
+    clean = attention.prompt_fn(oattn.to_device(data, "cuda"), splits=splits).view(new, -1)
+    data["qkv"][at, 9 * 128 + 70] = float("nan")
+    out = attention.prompt_fn(oattn.to_device(data, "cuda"), splits=splits).view(new, -1)
+    torch.cuda.synchronize()
+    abi.status_for("cuda").raise_if_set("nan")
+    bad = torch.tensor([j >= at and (window == 0 or j - at < window or 90 + at < sinks) for j in range(new)], device="cuda")
+    assert torch.isnan(out[bad].float()).all()
+    assert torch.equal(out[~bad], clean[~bad])
+
+
 def test_prompt_of_many_units_and_heads():
     """More units than SMs, in pairs and alone, with lengths that differ by far: every unit once."""
     for ctx, new in (([0] * 9, [700, 1, 64, 65, 300, 0, 129, 500, 33]), ([50] * 150, [1 + i % 7 for i in range(150)])):
