@@ -155,6 +155,23 @@ def test_prompt_rows_behind_the_last_request_stay():
     check(data, whole[:85, :2048].cpu(), k_new, v_new, "padded")
 
 
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("new", [20, 90])
+def test_prompt_rows_that_start_on_16_bytes_only(new, splits):
+    """Rows of qkv and out that lie at odd multiples of 16 bytes: the same bits as at 32."""
+    from muse_spark_open_b200 import abi, attention
+    data = make_prompt([150], [new], 15, window=70, sinks=2, wide=8)
+    dev = oattn.to_device(data, "cuda")
+    want = attention.prompt_fn(dict(dev, qkv=dev["qkv"][:, :-8].contiguous()), splits=splits)
+    for width, at in ((2048 + 8, 0), (2048 + 24, 8), (2048 + 16, 8)):
+        whole = torch.full((new, width), 7.0, dtype=torch.bfloat16, device="cuda")
+        attention.prompt_fn(dev, out=whole[:, at:at + 2048], splits=splits)
+        torch.cuda.synchronize()
+        abi.status_for("cuda").raise_if_set("attention")
+        assert torch.equal(whole[:, at:at + 2048], want)
+        assert (whole[:, :at] == 7.0).all() and (whole[:, at + 2048:] == 7.0).all()
+
+
 def test_prompt_leaves_other_pages_alone_and_replays_bitwise():
     data = make_prompt([100, 0, 77], [65, 33, 1], 6)
     before = data["k_cache"].view(torch.uint8).clone()
