@@ -165,8 +165,9 @@ int msk_attn_prompt_scratch_bytes(const MskPromptParams* p, size_t* bytes);
  * branch them, take pages back, and defragment.  All state is on the device and changed in place; nothing is read back, so
  * every call can be captured.  `refs[p]` is the number of page-table entries that name page p; a page is free when it is 0.
  * New pages are the lowest free ones, given out in the order of the call's rows.  Calls on one pool are ordered by their
- * stream.  A row or page index out of range, a row that one call lists twice (extend, fork), a child that is also a parent:
- * MSK_ERR_BOUNDS in `status`, and that entry is skipped.  No free page, or more tokens than max_pages hold:
+ * stream.  A row or page index out of range, a row that one call lists twice (extend, fork), a child that is also a parent,
+ * new tokens that would go into a page which other rows share (seq_lens was set back behind a fork): MSK_ERR_BOUNDS in
+ * `status`, and that entry is skipped.  No free page, or more tokens than max_pages hold:
  * MSK_ERR_CAPACITY, and the positions concerned get no page (fork: the child is left empty).
  * The reference has no counterpart: its inputs come with a finished page table (muse_attention_decode/reference.py:168-253).
  */

@@ -154,6 +154,9 @@ __device__ __forceinline__ void span_of(const PlanArgs& p, int row, int j, int* 
     }
 }
 
+// A page that new tokens of a row must not go into: another row holds it too, or there is no such page.
+__device__ __forceinline__ bool not_its_own(const PlanArgs& p, int id) { return id >= p.num_pages || (id >= 0 && __ldcg(p.refs + id) > 1); }
+
 // One CTA or one cluster: gives list entries the free pages they need.  kFork: one page for a child whose parent ends inside a page.
 template <bool kFork>
 __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
@@ -217,8 +220,14 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
                 const int last = static_cast<int>((static_cast<long long>(seq) + p.q_len - 1) >> p.page_log);
                 if (ok && p.q_len > 0 && last >= p.max_pages) report(p.status, MSK_ERR_CAPACITY, kWhere | 3, last, p.max_pages);
                 if (ok && p.q_len > 0)
-                    for (int lp = seq >> p.page_log; lp <= min(last, p.max_pages - 1); ++lp)
-                        need += p.page_table[static_cast<size_t>(row) * p.max_pages + lp] < 0;
+                    for (int lp = seq >> p.page_log; lp <= min(last, p.max_pages - 1); ++lp) {
+                        const int id = p.page_table[static_cast<size_t>(row) * p.max_pages + lp];
+                        need += id < 0;
+                        if (not_its_own(p, id)) {
+                            report(p.status, MSK_ERR_BOUNDS, kWhere | 7, id, row);
+                            ok = false;
+                        }
+                    }
             } else {
                 report(p.status, MSK_ERR_BOUNDS, kWhere | 2, row, j);
             }
@@ -240,8 +249,11 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
                 const int end = ok ? min(last, p.max_pages - 1) : first - 1;
                 for (int lp0 = first; lp0 <= end; lp0 += 32) {
                     const int lp = lp0 + lane;
-                    const bool want = lp <= end && p.page_table[static_cast<size_t>(row) * p.max_pages + lp] < 0;
-                    need += __popc(__ballot_sync(0xffffffffu, want));
+                    const int id = lp <= end ? p.page_table[static_cast<size_t>(row) * p.max_pages + lp] : 0x80000000;
+                    need += __popc(__ballot_sync(0xffffffffu, lp <= end && id < 0));
+                    const uint32_t bad = __ballot_sync(0xffffffffu, not_its_own(p, id));
+                    if (bad != 0 && lane == __ffs(bad) - 1) report(p.status, MSK_ERR_BOUNDS, kWhere | 7, id, row);
+                    ok = ok && bad == 0;
                 }
             }
             if (lane == 0) p.need[j] = ok ? need : -1;

@@ -15,7 +15,8 @@ that uses the pool.  A step of a serving loop:
 Everything happens on the device, in place and in stream order (order the streams yourself when you use several on one pool);
 nothing is read back, so all calls can be captured in a CUDA
 graph.  New pages are the lowest free ones, given out in the order of the rows: results do not depend on scheduling.
-Problems with the contents (a row out of range or listed twice, no free page) are reported in the status word
+Problems with the contents (a row out of range or listed twice, no free page, seq_lens set back into pages that a fork shares
+and then extended) are reported in the status word
 (`abi.status_for(device).raise_if_set()`), and the entries concerned are skipped; include/msk.h says how.
 The reference has no counterpart: its inputs come with a finished table (muse_attention_decode/reference.py:168-253).
 """
@@ -61,13 +62,15 @@ def _scratch(pool: dict, q: bytes, shape, n: int):
     counts and are ordered anyway.  Lists longer than the pool has rows (and a first call inside a graph capture, whose memory
     is the graph's) get memory of their own, for the call."""
     kept = pool.get("scratch")
-    if kept is not None and kept[0] == shape and n <= shape[0]:
+    if kept is not None and (kept[0] != shape or kept[4] is not pool["refs"]):
+        kept = None  # a copy of another pool's dict, with counts of its own
+    if kept is not None and n <= shape[0]:
         return kept[1], kept[2], None
     b = C.c_size_t()
     abi.check(abi.lib().msk_pages_scratch_bytes(q, max(n, shape[0]), C.byref(b)), "msk_pages_scratch_bytes")
     t = torch.empty(b.value, dtype=torch.uint8, device=pool["refs"].device)
     if kept is None and n <= shape[0] and not torch.cuda.is_current_stream_capturing():
-        pool["scratch"] = (shape, t.data_ptr(), b.value, t)
+        pool["scratch"] = (shape, t.data_ptr(), b.value, t, pool["refs"])
     return t.data_ptr(), b.value, t
 
 

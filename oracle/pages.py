@@ -37,6 +37,11 @@ class Pool:
                 bad.add("bounds")
                 loc += [-1] * n
                 continue
+            span = {pos // self.size for pos in range(self.seq[r], self.seq[r] + n)}
+            if any(self.refs[self.table[r][lp]] > 1 for lp in span if lp < self.max_pages and self.table[r][lp] >= 0):
+                bad.add("bounds")  # a page that other rows share
+                loc += [-1] * n
+                continue
             for pos in range(self.seq[r], self.seq[r] + n):
                 lp = pos // self.size
                 if lp >= self.max_pages:

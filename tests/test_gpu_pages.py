@@ -192,3 +192,46 @@ def test_nothing_to_do():
     assert pages.compact(pool, [cache]).tolist() == [0, 0]
     pages.fork(pool, i32([0]), i32([1]), [])  # an empty parent, no caches
     assert not status() and not pool["refs"].any() and (pool["page_table"] == -1).all()
+
+
+@pytest.mark.parametrize("num_pages", [40, 20000])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_tokens_do_not_go_into_a_page_that_a_fork_shares(num_pages, ragged):
+    """seq_lens set back behind a fork: the rows that would write into a shared page are refused, the others get theirs;
+    once the other holder is gone, the same call goes through."""
+    from muse_spark_open_b200 import pages
+    model = Pool(num_pages, 16, 5, 40)
+    for row, n in enumerate([40, 64, 10]):
+        model.extend([row], [n])
+        model.seq[row] = n
+    pool, caches, dev = upload(model, [(2, 16)])
+    pages.fork(pool, i32([0, 1]), i32([3, 4]), dev)
+    model.fork([0, 1], [3, 4], caches)
+    # row 0: into the second of two shared pages; row 4: ends in front of its shared ones; row 3: behind them, in its own page
+    for row, n in ((0, 20), (4, 64), (1, 0)):
+        model.seq[row] = n
+        pool["seq_lens"][row] = n
+    counts = [8, 8, 8, 8, 8] if not ragged else [8, 300, 0, 5, 3]
+    cu = i32([0, *torch.tensor(counts).cumsum(0).tolist()]) if ragged else None
+    for gone in (None, 3, 4):
+        if gone is not None:
+            pages.free(pool, i32([gone]))
+            model.free([gone])
+        rows = [0, 1, 2, 3, 4]
+        loc = pages.extend(pool, i32(rows), 8) if not ragged else pages.extend(pool, i32(rows), 1, cu, sum(counts))
+        want, bad = model.extend(rows, counts)
+        assert loc.tolist() == want and status() == bad and ("bounds" in bad) == (gone != 4)
+        same(model, pool, caches, dev)
+
+
+def test_a_copied_pool_has_a_workspace_of_its_own():
+    from muse_spark_open_b200 import pages
+    pool = pages.prepare(64, 16, 4, 8)
+    pages.extend(pool, i32([0, 1]), 20)
+    twin = dict(pool, **{k: pool[k].clone() for k in ("page_table", "seq_lens", "refs")})
+    pages.extend(twin, i32([2]), 20)
+    assert twin["scratch"][1] != pool["scratch"][1]
+    first = pool["scratch"][1], twin["scratch"][1]
+    pages.extend(twin, i32([3]), 20)
+    pages.extend(pool, i32([3]), 20)
+    assert first == (pool["scratch"][1], twin["scratch"][1]) and not status()

@@ -71,3 +71,17 @@ def test_refusals():
                 lambda: pages.free(dict(pool, refs=pool["refs"].long()), rows), lambda: pages.prepare(10, 12, 4, 4, device="cpu")):
         with pytest.raises(abi.MskError):
             bad()
+
+
+def test_model_refuses_tokens_in_shared_pages():
+    pool = Pool(20, 8, 3, 6)
+    pool.extend([0], [20])
+    pool.seq[0] = 20
+    assert not pool.fork([0], [1], [])
+    pool.seq[0] = 12                           # back into the second page, which row 1 holds too
+    assert pool.extend([0], [4]) == ([-1] * 4, {"bounds"})
+    pool.seq[0] = 16                           # behind the shared pages: its own page
+    assert pool.extend([0], [4])[1] == set()
+    pool.free([1])
+    pool.seq[0] = 12
+    assert pool.extend([0], [4])[1] == set()
