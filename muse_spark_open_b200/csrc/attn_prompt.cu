@@ -2,8 +2,9 @@
 // FP8-E4M3 cache, with a sliding window and first tokens that stay visible.  Two launches, three when the keys are split:
 //
 //   prep     one CTA per token: RMSNorm, scale and RoPE of its queries (rounded to BF16, kept as FP16 in the workspace) and
-//            keys; keys and values quantised to E4M3 and written into the pages the page table names.  One more CTA lists
-//            the work units (request, first token).  Bound by memory: 18 KB per token at 32 + 4 + 4 heads.
+//            keys; keys and values quantised to E4M3 and written into the pages the page table names.  Keys and angles are
+//            taken in 64 bits (2 us of 310 at 4096 tokens).  One more CTA lists the work units (request, first token), unless
+//            they are few and every CTA finds its own.  Bound by memory: 18 KB per token at 32 + 4 + 4 heads.
 //   main     one CTA, or a pair of CTAs on neighbouring SMs, per (unit of 32 or 64 new tokens, KV head, split): flash
 //            attention.  The 8 query heads of a KV head and the tokens together are the rows of the product: a CTA has 2
 //            tiles of 128 rows = 16 tokens x 8 heads.
@@ -21,6 +22,16 @@
 // The products run ahead of the softmax in halves of 64 keys: while the softmax works on one half of a row tile's scores,
 // the tensor cores add the other half's product and put the next tile's scores in its place.  (With whole tiles each tile
 // waited 1300 clocks for its next scores, a third of the loop; a third row tile does not fit.)
+// Values are 0 * V for the tokens that do not see them, so a NaN among them is zeroed where not all tokens of the unit see it,
+// and the rows that do are made NaN at the end.
+// Measured (32 + 4 heads): 8192 tokens, full, behind nothing: 539 us = 1.02 PFLOP/s, 62 % of the rate of a BF16 matrix product;
+// four prompts under windows 327 - 333 us, 0.49 PFLOP/s of visible keys; one follow-up question 20 us.  Bound by the softmax
+// warps' instruction issue: 1750 - 1850 clocks per 64 keys and two row tiles, of which a loop of the softmax alone takes 1500
+// (issue slots: two warps of softmax per scheduler, beside them the MMA, copying or converting warps); the tensor cores are
+// a third busy.  Per unit come 12 us: 3 until the first scores, 2 for the last product, 5.5 for norm, gate and stores, 1 until
+// the next CTA runs.  Under a window a unit has only 5 to 40 tiles, so these and the masked parts of its edge tiles weigh more.
+// Tried without gain: an MMA warp per row tile, a reference without a maximum, turn-taking softmax warps, scores fetched a
+// half ahead, a persistent grid, output tiles stored by TMA, four softmax warpgroups, more polynomials.
 // TMEM: S (P over the first half of each half) and O, 128 columns each, for two row tiles = all 512 columns.
 // Pairs (CG = 2, tcgen05 cta_group::2): a tile's products run over both SMs, 256 rows, each CTA bringing its rows and half of
 // the K and V tile.  A single CTA is bound by shared memory: per tile 128 KB of Q and K reads, 64 KB of V, 96 KB of
@@ -35,7 +46,7 @@ namespace {
 
 constexpr int kTile = 128;                  // keys per tile
 constexpr int kTok = 16;                    // tokens per row tile
-constexpr int kThreads = 512;               // softmax A | softmax B | converting | MMA, copying, two idle warps
+constexpr int kThreads = 512;               // softmax A | softmax B | converting | MMA, copying, one that waits for the queries, one idle
 constexpr int kQBytes = 32768;              // one row tile of queries: two swizzled halves of 64 channels
 template <int CG>
 struct Geo {
@@ -188,7 +199,7 @@ __global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
     };
     fetch(warp);
     const bool turn = p.inv_freq != nullptr;
-    const float2 freq = turn ? __ldg(reinterpret_cast<const float2*>(p.inv_freq) + lane) : make_float2(0.0f, 0.0f);
+    const float my_freq = turn && threadIdx.x < 64 ? __ldg(p.inv_freq + threadIdx.x) : 0.0f;
     const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
     // the request of token t: the last b with cu[b] <= t, by steps of 32 requests
     int lo = 0, hi = p.B;  // cu[lo] <= t < cu[hi] is looked for in [lo, hi)
@@ -204,24 +215,23 @@ __global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
     }
     const int b = lo;
     const int pos = p.seq_lens[b] + t - (p.cu != nullptr ? p.cu[b] : b * p.q_len);
-    float c[2] = {1.0f, 1.0f}, s[2] = {0.0f, 0.0f};
-    if (turn) {
-        const float fp = static_cast<float>(pos);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            // the product's rounding error (up to 5e-4 at position 8192) is put back to first order
-            const float f = h ? freq.y : freq.x, ang = fp * f, err = fmaf(fp, f, -ang);
-            float cs, sn;
-            sincosf(ang, &sn, &cs);
-            c[h] = cs - err * sn;
-            s[h] = sn + err * cs;
-        }
+    // cos and sin of the token's 64 angles, in 64 bits (a product in 32 bits is off by up to 5e-4 at position 8192)
+    __shared__ double2 angles[64];
+    if (turn && threadIdx.x < 64) {
+        double sn, cs;
+        sincos(static_cast<double>(pos) * static_cast<double>(my_freq), &sn, &cs);
+        angles[threadIdx.x] = make_double2(cs, sn);
     }
     const int page = pos >> p.page_log;
     const int id = pos >= 0 && page < p.max_pages ? p.page_table[static_cast<size_t>(b) * p.max_pages + page] : -1;
     const bool page_ok = id >= 0 && id < p.num_pages;
     if (!page_ok && threadIdx.x == 0) report(p.status, MSK_ERR_BOUNDS, MSK_K_PROMPT << 8 | 2, id, page);
     const size_t slot = page_ok ? (static_cast<size_t>(id) << p.page_log) + (pos & (p.page_size - 1)) : 0;
+    __syncthreads();
+    double2 turn2[2] = {make_double2(1.0, 0.0), make_double2(1.0, 0.0)};
+    if (turn) turn2[0] = angles[2 * lane], turn2[1] = angles[2 * lane + 1];
+    const float c[2] = {static_cast<float>(turn2[0].x), static_cast<float>(turn2[1].x)};
+    const float s[2] = {static_cast<float>(turn2[0].y), static_cast<float>(turn2[1].y)};
     for (int h0 = warp; h0 < heads; h0 += 8 * U) {
         if (h0 != warp) fetch(h0);
 #pragma unroll
@@ -240,10 +250,24 @@ __global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
                     make_uint2(*reinterpret_cast<uint32_t*>(&a[0]), *reinterpret_cast<uint32_t*>(&a[1]));
             } else {
                 const bool key = h < p.Hq + p.Hkv;
-                if (key) norm_turn(x, 1.0f, c, s, turn);
-                const float sc = key ? k_scale : v_scale;
-                const uint32_t w = f2_to_e4m3x2(__fdiv_rn(x[0], sc), __fdiv_rn(x[1], sc)) |
-                                   f2_to_e4m3x2(__fdiv_rn(x[2], sc), __fdiv_rn(x[3], sc)) << 16;
+                if (key) {
+                    // in 64 bits up to the quantisation: in 32 a few bytes of a million fall to the other side of a rounding
+                    // border, 6 % off
+                    const double a[4] = {x[0], x[1], x[2], x[3]};
+                    double ss = a[0] * a[0] + a[1] * a[1] + a[2] * a[2] + a[3] * a[3];
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const double r = 1.0 / (sqrt(ss * (1.0 / 128.0) + 1e-5) * static_cast<double>(k_scale));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        x[2 * i] = static_cast<float>((a[2 * i] * turn2[i].x - a[2 * i + 1] * turn2[i].y) * r);
+                        x[2 * i + 1] = static_cast<float>((a[2 * i] * turn2[i].y + a[2 * i + 1] * turn2[i].x) * r);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = __fdiv_rn(x[i], v_scale);
+                }
+                const uint32_t w = f2_to_e4m3x2(x[0], x[1]) | f2_to_e4m3x2(x[2], x[3]) << 16;
                 const int kv = h - p.Hq - (key ? 0 : p.Hkv);
                 if (page_ok)
                     *reinterpret_cast<uint32_t*>((key ? p.k_cache : p.v_cache) + (slot * p.Hkv + kv) * 128 + 4 * lane) = w;

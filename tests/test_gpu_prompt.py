@@ -155,6 +155,24 @@ def test_prompt_rows_behind_the_last_request_stay():
     check(data, whole[:85, :2048].cpu(), k_new, v_new, "padded")
 
 
+@pytest.mark.parametrize("ctx", [0, 20000])
+def test_prompt_keys_are_rounded_once(ctx):
+    """The cached keys and values are the 64-bit formula's, byte for byte, at far positions too."""
+    data = make_prompt([ctx], [700], 21, window=100, sinks=3)
+    _, k_new, v_new, _ = run(data)
+    cfg = data["config"]
+    q, k, v, _ = data["qkv"].double().split([16 * 128, 2 * 128, 2 * 128, 16 * 128], 1)
+    k, v = k.reshape(700, 2, 128), v.reshape(700, 2, 128)
+    k = k / torch.sqrt((k * k).mean(-1, keepdim=True) + 1e-5)
+    freq = (1.0 / (cfg["rope_theta"] ** (torch.arange(0, 128, 2).float() / 128))).double()
+    ang = (ctx + torch.arange(700).double())[:, None, None] * freq
+    a, b = k[..., 0::2], k[..., 1::2]
+    k = torch.stack((a * ang.cos() - b * ang.sin(), a * ang.sin() + b * ang.cos()), -1).flatten(-2)
+    for got, want in ((k_new, k / data["k_scale"].double()), (v_new, v / data["v_scale"].double())):
+        want = want.clamp(-448, 448).float().to(FP8).view(torch.uint8)
+        assert torch.equal(got.view(torch.uint8).view(want.shape), want)
+
+
 @pytest.mark.parametrize("splits", [1, 2])
 @pytest.mark.parametrize("new", [20, 90])
 def test_prompt_rows_that_start_on_16_bytes_only(new, splits):
