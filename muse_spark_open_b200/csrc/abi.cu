@@ -4,7 +4,7 @@
 #include "msk.h"
 #include "status.cuh"
 
-extern "C" int msk_version(void) { return 100; }
+extern "C" int msk_version(void) { return 101; }
 
 extern "C" int msk_device_info(int* sm_count, int* l2_bytes) {
     int dev = 0;

@@ -25,7 +25,8 @@
 // Values are 0 * V for the tokens that do not see them, so a NaN among them is zeroed where not all tokens of the unit see it,
 // and the rows that do are made NaN at the end.
 // Measured (32 + 4 heads): 8192 tokens, full, behind nothing: 539 us = 1.02 PFLOP/s, 62 % of the rate of a BF16 matrix product;
-// four prompts under windows 327 - 333 us, 0.49 PFLOP/s of visible keys; one follow-up question 20 us.  Bound by the softmax
+// three documents of 2500 to 4099 tokens under window 1024 + 64 sinks 330 us, 0.49 PFLOP/s of visible keys; 19 tokens behind
+// 7001 cached ones 20 us.  Bound by the softmax
 // warps' instruction issue: 1750 - 1850 clocks per 64 keys and two row tiles, of which a loop of the softmax alone takes 1500
 // (issue slots: two warps of softmax per scheduler, beside them the MMA, copying or converting warps); the tensor cores are
 // a third busy.  Per unit come 12 us: 3 until the first scores, 2 for the last product, 5.5 for norm, gate and stores, 1 until
