@@ -374,12 +374,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int W = p.window, snk = W > 0 ? p.sinks : 0;
     int t_first, sink_tiles;
     const int tiles = key_tiles(p, p_first, p_last, &t_first, &sink_tiles);
-    const int gap = t_first - sink_tiles;
+    const int win_tiles = tiles - sink_tiles;  // these first: their many keys set the references that the sinks' few would set too low
     const int per = (tiles + p.splits - 1) / p.splits;
     const int v_begin = sp * per;
     const int nt = n_tok > 0 ? max(0, min(per, tiles - v_begin)) : 0;
     const bool two = n_tok > kTok * CG;                    // the second row tile has tokens
-    auto base_of = [&](int i) { return (v_begin + i + (v_begin + i >= sink_tiles ? gap : 0)) * kTile; };
+    auto base_of = [&](int i) { return (v_begin + i + (v_begin + i < win_tiles ? t_first : -win_tiles)) * kTile; };
     auto tok_of = [&](int g) { return kTok * (CG * g + rank); };  // first token of row tile g here, within the unit
 
     tc_fence_before();
@@ -439,8 +439,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float tops = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
                 const bool move = tops - m > kLazy;
                 if (__any_sync(0xffffffffu, move)) {
-                    const float m_new = move ? tops + kAhead : m;
-                    const float alpha = move ? ex2(m - m_new) : 1.0f;
+                    // all of the warp's rows move up, not only those that must: four sinks first leave 32 low references, and
+                    // one of the rows outgrew its own in most of the following steps
+                    const float m_new = fmaxf(m, tops + kAhead);
+                    const float alpha = ex2(m - m_new);
                     m = m_new;
                     l *= alpha;
                     if (t > 0) {  // the accumulator follows, once the last product has been added
