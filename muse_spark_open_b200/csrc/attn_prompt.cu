@@ -342,17 +342,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (tid == 64) prefetch_tmap(&tm_q), prefetch_tmap(&tm_k), prefetch_tmap(&tm_v);
     if (warp == 0) tmem_alloc_cg<CG>(smem_u32(&tmem_slot), 512);
-    pdl_wait();
+    // Where a CTA finds its unit itself, only the copying warp waits for the prep kernel, with the first tiles of old keys on
+    // their way: what came before the prep kernel is complete (it waits for that before it lets this one start).
+    if (!p.direct) pdl_wait();
     pdl_launch_dependents();
 
     // ---------------- this CTA's unit: the pair's row tile g covers tokens 16 CG g .. of the unit, this CTA 16 of them
     int4 u = make_int4(0, 0, 0, 0);  // request, first row, tokens, first position
+    int old_end = 0;                 // positions below are older than this call (known to direct units)
     if (!p.direct) {
         const int n_units = __ldcg(p.units);
         if (slot_u < n_units) u = __ldcg(reinterpret_cast<const int4*>(p.units + kMaxUnitsHeader + 4 * slot_u));
     } else if (p.cu == nullptr) {
         const int per_req = (p.q_len + p.unit - 1) / p.unit, rb = slot_u / per_req, at = (slot_u - rb * per_req) * p.unit;
-        if (rb < p.B) u = make_int4(rb, rb * p.q_len + at, min(p.q_len - at, p.unit), p.seq_lens[rb] + at);
+        if (rb < p.B) {
+            old_end = p.seq_lens[rb];
+            u = make_int4(rb, rb * p.q_len + at, min(p.q_len - at, p.unit), old_end + at);
+        }
     } else {  // a lane per request (B <= 32): which one's groups of tokens hold number slot_u
         const int n = lane < p.B ? new_tokens(p, lane) : 0, row0 = lane < p.B ? first_row(p, lane) : 0, seq = lane < p.B ? p.seq_lens[lane] : 0;
         const int groups = (n + p.unit - 1) / p.unit;
@@ -366,8 +372,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (behind != 0) {
             const int src = __ffs(behind) - 1;
             const int at = (slot_u - (__shfl_sync(0xffffffffu, inc, src) - __shfl_sync(0xffffffffu, groups, src))) * p.unit;
-            u = make_int4(src, __shfl_sync(0xffffffffu, row0, src) + at, min(__shfl_sync(0xffffffffu, n, src) - at, p.unit),
-                          __shfl_sync(0xffffffffu, seq, src) + at);
+            old_end = __shfl_sync(0xffffffffu, seq, src);
+            u = make_int4(src, __shfl_sync(0xffffffffu, row0, src) + at, min(__shfl_sync(0xffffffffu, n, src) - at, p.unit), old_end + at);
         }
     }
     const int b = u.x, tok0 = u.y, n_tok = u.z, p_first = u.w, p_last = p_first + max(n_tok, 1) - 1;
@@ -717,12 +723,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         } else if (warp == 13 && nt > 0) {
             // ================ the copying warp
-            if (lane == 0) {
-                mbar_expect_tx(q_here, (two ? 2 : 1) * kQBytes);
-                for (int g = 0; g < (two ? 2 : 1); ++g)
-                    for (int c = 0; c < 2; ++c)
-                        tma_load_3d(s_q + g * kQBytes + c * 16384, &tm_q, q_here, 64 * c, h * 8, tok0 + tok_of(g));
-            }
             const int ppt = kTile >> p.page_log;  // pages per tile, <= 16: lane j fetches page j
             auto page_of = [&](int i) {
                 const int pg = (base_of(i) >> p.page_log) + lane;
@@ -738,29 +738,49 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool k_mine = lane < ppt && (CG == 1 || p.page_size == kTile || (key0 >= rank * G::kKeys && key0 < (rank + 1) * G::kKeys));
             const int k_in_page = CG == 2 && p.page_size == kTile ? rank * G::kKeys : 0;
             const uint32_t k_at = CG == 2 ? (p.page_size == kTile ? 0 : key0 - rank * G::kKeys) * 128 : key0 * 128;
-            int id = page_of(0);
+            auto fetch = [&](int kv, int stage, int id) {
+                const uint32_t full = st_full + 8 * (kv * SS + stage), dst = s_f8 + (kv * SS + stage) * G::kF8;
+                if (lane == 0) mbar_expect_tx(full, G::kF8);
+                __syncwarp();
+                if (kv == 0) {
+                    if (k_mine) tma_load_4d(dst + k_at, &tm_k, full, 0, h, k_in_page, id);
+                } else {
+                    if (lane < ppt) tma_load_4d(dst + key0 * G::kChan, &tm_v, full, CG == 2 ? rank * G::kChan : 0, h, 0, id);
+                }
+            };
+            int id = page_of(0), i = 0;
             bool ok = true;
             int stage = 0, ph = 0;
-            for (int i = 0; i < nt && ok; ++i) {
+            if (p.direct) {
+                for (; i < SS && i < nt && base_of(i) + kTile <= old_end; ++i) {
+                    const int next = i + 1 < nt ? page_of(i + 1) : -1;
+                    fetch(0, stage, id);
+                    fetch(1, stage, id);
+                    id = next;
+                    if (++stage == SS) stage = 0, ph ^= 1;
+                }
+                pdl_wait();
+            }
+            if (lane == 0) {
+                mbar_expect_tx(q_here, (two ? 2 : 1) * kQBytes);
+                for (int g = 0; g < (two ? 2 : 1); ++g)
+                    for (int c = 0; c < 2; ++c)
+                        tma_load_3d(s_q + g * kQBytes + c * 16384, &tm_q, q_here, 64 * c, h * 8, tok0 + tok_of(g));
+            }
+            for (; i < nt && ok; ++i) {
                 const int next = i + 1 < nt ? page_of(i + 1) : -1;
                 for (int kv = 0; kv < 2; ++kv) {
-                    const uint32_t full = st_full + 8 * (kv * SS + stage);
                     if (i >= SS) ok = mbar_wait(st_free + 8 * (kv * SS + stage), ph ^ 1, p.status, where | 14) && ok;
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(full, G::kF8);
-                    __syncwarp();
-                    const uint32_t dst = s_f8 + (kv * SS + stage) * G::kF8;
-                    if (kv == 0) {
-                        if (k_mine) tma_load_4d(dst + k_at, &tm_k, full, 0, h, k_in_page, id);
-                    } else {
-                        if (lane < ppt) tma_load_4d(dst + key0 * G::kChan, &tm_v, full, CG == 2 ? rank * G::kChan : 0, h, 0, id);
-                    }
+                    fetch(kv, stage, id);
                 }
                 id = next;
                 if (++stage == SS) stage = 0, ph ^= 1;
             }
             __syncwarp();
+        } else if (warp == 13) {
+            if (p.direct) pdl_wait();  // no CTA ends before the prep kernel does
         } else if (warp == 14 && nt > 0) {
             // ================ this CTA's queries have arrived: tell the MMA warp
             const bool ok = mbar_wait(q_here, 0, p.status, where | 15);
