@@ -147,7 +147,7 @@ typedef struct {
     const float* inv_freq;    /* [d/2] or NULL */
     int B, T, Hq, Hkv, d, page_size, num_pages, window, sinks;
     float qk_scale_factor, sm_scale;
-    int splits;               /* ways the keys of a unit of 32 tokens are split over CTAs, up to 64; 0 = pick */
+    int splits;               /* ways the keys of a unit (32 or 64 tokens) are split over CTAs, up to 64; 0 = pick */
     int pdl;                  /* chain the first kernel to whatever precedes it */
     void* scratch;            /* msk_attn_prompt_scratch_bytes(), 256-byte aligned, any contents; launches that may overlap on
                                  the GPU need one each */

@@ -872,12 +872,17 @@ int plan_prompt(const MskPromptParams* q, Plan* plan) {
     }
     plan->splits = q->splits;
     if (q->splits == 0) {
-        // fewer units than SMs: the keys are split, down to two tiles a piece
+        // Fewer units than SMs: the keys are split into pieces of equal tiles, as many as find an SM, down to one tile.  Parts
+        // cost their way through memory, a tile's time for some 3500 rows (token, head): 300 tokens x 32 heads over 3 tiles take
+        // 21.0 us whole and 22.3 in three pieces, over 5 tiles 24.8 and 24.0; 8 tokens over 5 tiles 14.9 and 11.1.
         const long long ctas = static_cast<long long>(plan->max_units) * q->Hkv * plan->cg;
-        long long s = 148 / ctas;
-        if (s > (tiles + 1) / 2) s = (tiles + 1) / 2;
-        if (s > 32) s = 32;
-        plan->splits = s < 1 ? 1 : static_cast<int>(s);
+        long long most = 148 / ctas;
+        if (most > 32) most = 32;
+        plan->splits = 1;
+        if (most > 1) {
+            const long long per = (tiles + most - 1) / most;
+            if ((tiles - per) * 3500 > static_cast<long long>(q->T) * q->Hq) plan->splits = static_cast<int>((tiles + per - 1) / per);
+        }
     }
     auto up = [](size_t v) { return (v + 255) & ~static_cast<size_t>(255); };
     const size_t rows = static_cast<size_t>(q->T) * q->Hq;
