@@ -67,14 +67,15 @@ def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
             data["cache_loc"].dtype != torch.int64:
         raise abi.MskError("seq_lens / page_table must be int32 and cache_loc int64")
     if qkv.is_contiguous() and b * l > 0 and qkv.numel() % (b * l) == 0:
-        ld = qkv.numel() // (b * l)
+        cols = ld = qkv.numel() // (b * l)
     else:
-        ld = qkv.view(b * l, -1).stride(0)
+        flat = qkv.view(b * l, -1)
+        cols, ld = flat.shape[1] if flat.stride(1) == 1 else 0, flat.stride(0)
     out = torch.empty((b, l, wide), dtype=torch.bfloat16, device=qkv.device)
     if l != 1 and (l != 8 or cfg.get("sinks", 0)) and not chunks and not stages:
         # blocks of other lengths, and verify blocks with sinks: the prompt kernels (16 requests x 8 tokens, window 1024 + 4
         # sinks: 24 us against 51 us for the verify kernel, whose results without sinks stay what they were)
-        _run_prompt(data, cfg, qkv.view(b * l, -1) if ld != qkv.stride(0) else qkv, out.view(b * l, wide), None, l, 0)
+        _run_prompt(data, cfg, qkv, b * l, cols, ld, out, wide, None, l, 0)
         return out
     _run_step(abi.ptr(qkv), ld, out.data_ptr(), wide, data, cfg, qkv.get_device(), chunks, stages, 0, False, 0)
     return out
@@ -83,14 +84,15 @@ def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
 _prompt_bytes: dict = {}
 
 
-def _run_prompt(data: dict, cfg: dict, qkv: torch.Tensor, out: torch.Tensor | None, cu: torch.Tensor | None, q_len: int, splits: int) -> torch.Tensor:
-    """msk_attn_prompt on checked arguments; cu None: q_len tokens per request."""
+def _run_prompt(data: dict, cfg: dict, qkv: torch.Tensor, t: int, cols: int, ld_qkv: int, out: torch.Tensor | None, ld_out: int,
+                cu: torch.Tensor | None, q_len: int, splits: int) -> torch.Tensor:
+    """msk_attn_prompt on checked arguments: t rows of `cols` values in qkv (0: not such rows), ld_qkv apart; cu None: q_len
+    tokens per request; out None: made here."""
     kc, vc, table, seq, ks, vs = data["k_cache"], data["v_cache"], data["page_table"], data["seq_lens"], data["k_scale"], data["v_scale"]
     b, hq, hkv, d, page = cfg["batch"], cfg["num_q_heads"], cfg["num_kv_heads"], cfg["head_dim"], cfg["page_size"]
     if qkv.dtype != torch.bfloat16 or kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn:
         raise abi.MskError("qkv must be bfloat16 and the cache float8_e4m3fn")
-    t, wide = qkv.shape if qkv.dim() == 2 else (0, 0)
-    if wide < (2 * hq + 2 * hkv) * d or qkv.stride(1) != 1:
+    if cols < (2 * hq + 2 * hkv) * d:
         raise abi.MskError("qkv must be [tokens, (2Hq+2Hkv)*d] with unit column stride")
     if seq.dtype != torch.int32 or table.dtype != torch.int32 or (cu is not None and cu.dtype != torch.int32):
         raise abi.MskError("seq_lens / page_table / cu_seqlens_q must be int32")
@@ -106,9 +108,7 @@ def _run_prompt(data: dict, cfg: dict, qkv: torch.Tensor, out: torch.Tensor | No
     index = abi.here((qkv, kc, vc, ks, vs, seq, table) if cu is None else (qkv, kc, vc, ks, vs, seq, table, cu))
     dev = qkv.device
     if out is None:
-        out = torch.empty((t, hq * d), dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.shape != (t, hq * d) or out.stride(1) != 1:
-        raise abi.MskError("out must be bfloat16 [tokens, Hq*d] with unit column stride")
+        out, ld_out = torch.empty((t, hq * d), dtype=torch.bfloat16, device=dev), hq * d
     elif out.get_device() != index:
         raise abi.MskError("the tensors of one call must be on one device")
     if t == 0:
@@ -132,7 +132,7 @@ def _run_prompt(data: dict, cfg: dict, qkv: torch.Tensor, out: torch.Tensor | No
         nbytes = _prompt_bytes[key] = n.value
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     args = _prompt_args.pack(
-        qkv.data_ptr(), qkv.stride(0), out.data_ptr(), out.stride(0), kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), seq.data_ptr(),
+        qkv.data_ptr(), ld_qkv, out.data_ptr(), ld_out, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), seq.data_ptr(),
         0 if cu is None else cu.data_ptr(), table.data_ptr(), max_pages, freq, b, t, hq, hkv, d, page, pages, window, sinks,
         cfg["qk_scale_factor"], cfg["sm_scale"], splits, 0, scratch.data_ptr(), nbytes, q_len)
     rc = lib.msk_attn_prompt(args, abi.status_ptr(index), abi.raw_stream(index))
@@ -150,4 +150,8 @@ def prompt_fn(data: dict, out: torch.Tensor | None = None, splits: int = 0) -> t
     (a padded batch) are not touched: they keep what `out` held.  The workspace comes from torch's allocator on the current
     stream, so calls on several streams or in several captured graphs do not share it.
     """
-    return _run_prompt(data, data["config"], data["qkv"], out, data["cu_seqlens_q"], 0, splits)
+    cfg, qkv = data["config"], data["qkv"]
+    t, cols = qkv.shape if qkv.dim() == 2 and qkv.stride(1) == 1 else (0, 0)
+    if out is not None and (out.dtype != torch.bfloat16 or out.shape != (t, cfg["num_q_heads"] * cfg["head_dim"]) or out.stride(1) != 1):
+        raise abi.MskError("out must be bfloat16 [tokens, Hq*d] with unit column stride")
+    return _run_prompt(data, cfg, qkv, t, cols, qkv.stride(0) if cols else 0, out, 0 if out is None else out.stride(0), data["cu_seqlens_q"], 0, splits)
