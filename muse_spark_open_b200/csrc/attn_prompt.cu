@@ -89,6 +89,7 @@ struct PromptArgs {
     int max_pages;
     const float* inv_freq;
     int B, T, Hq, Hkv, page_size, page_log, num_pages, window, sinks, splits, max_units;
+    int last_tile;    // of the page table
     int out_wide;     // rows of out allow 32-byte stores
     float qk_scale_factor, q_scale, s_scale;  // queries are stored times q_scale (a power of two); scores times s_scale * k_scale
     __half* q16;      // [T, Hq, 128]
@@ -122,12 +123,14 @@ __device__ __forceinline__ void norm_turn(float (&x)[4], float post_scale, const
     }
 }
 
-// How many key tiles a unit's tokens see, and where they are: [0, sink_tiles) and [first, first + tiles - sink_tiles).
+// How many key tiles a unit's tokens see, and where they are: [0, sink_tiles) and [first, first + tiles - sink_tiles).  None lie
+// behind the page table's last one, whatever seq_lens says (the prep kernel reports it).
 __device__ __forceinline__ int key_tiles(const PromptArgs& p, int p_first, int p_last, int* first, int* sink_tiles) {
     const int W = p.window, snk = W > 0 ? p.sinks : 0;
-    *first = (W > 0 ? max(0, p_first - W + 1) : 0) / kTile;
-    *sink_tiles = min((min(snk, p_last + 1) + kTile - 1) / kTile, *first);
-    return p_last / kTile - *first + 1 + *sink_tiles;
+    *first = (W > 0 && p_first >= W ? p_first - W + 1 : 0) / kTile;
+    const int last = min(p_last / kTile, p.last_tile);
+    *sink_tiles = min(min(snk / kTile + (snk % kTile != 0), *first), last + 1);
+    return last - *first + 1 + *sink_tiles;
 }
 
 // The unit list: each request's new tokens in groups of p.unit, the units with the most key tiles first (a counting sort over
@@ -936,6 +939,7 @@ extern "C" int msk_attn_prompt(const MskPromptParams* q, int* status, void* stre
     a.page_table = q->page_table, a.max_pages = q->max_pages, a.inv_freq = q->inv_freq;
     a.B = q->B, a.T = q->T, a.Hq = q->Hq, a.Hkv = q->Hkv, a.page_size = q->page_size, a.num_pages = q->num_pages;
     while ((1 << a.page_log) < q->page_size) ++a.page_log;
+    a.last_tile = static_cast<int>((static_cast<long long>(q->max_pages) * q->page_size - 1) / kTile);
     a.window = q->window, a.sinks = q->sinks, a.splits = plan.splits, a.max_units = plan.max_units, a.unit = 2 * kTok * plan.cg;
     a.out_wide = ((reinterpret_cast<uintptr_t>(q->out) | static_cast<uintptr_t>(q->ld_out) * 2) & 31) == 0;
     a.qk_scale_factor = q->qk_scale_factor;

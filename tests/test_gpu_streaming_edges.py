@@ -125,6 +125,23 @@ def test_page_ids_and_positions_that_do_not_exist():
         abi.status_for("cuda").raise_if_set("past the table")
 
 
+@pytest.mark.parametrize("seq", [2 ** 31 - 1, 2 ** 31 - 40, 10 ** 9, 500, -1, -500, -2 ** 31])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 0), (100, 2 ** 31 - 1), (2 ** 31 - 1, 7)])
+def test_lengths_that_no_request_can_have(seq, window, sinks):
+    """One request's length is nonsense: reported, at once, and the other requests are what they were."""
+    from muse_spark_open_b200 import abi, attention
+    for new in ([50, 40, 30], [9, 7, 8]):
+        data = make_prompt([130, 60, 0], new, 12, hkv=1, window=window, sinks=sinks)
+        good = attention.prompt_fn(oattn.to_device(data, "cuda"))
+        data["seq_lens"][1] = seq
+        out = attention.prompt_fn(oattn.to_device(data, "cuda"))
+        torch.cuda.synchronize()
+        with pytest.raises(abi.MskError, match="out of range in attn_prompt"):
+            abi.status_for("cuda").raise_if_set("length")
+        a, b = new[0], new[0] + new[1]
+        assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])
+
+
 @pytest.mark.parametrize("splits", [1, 2])
 @pytest.mark.parametrize("new", [40, 20])  # pairs of CTAs, and single ones
 @pytest.mark.parametrize("at", [0, 1, 5, 6, 7, 38, 70, 127, 150])
