@@ -1,7 +1,8 @@
 // Gated attention decode (L = 1) and 8-token verify (L = 8) over a paged FP8-E4M3 KV cache, one launch.
 //
 // Grid (chunks C, KV heads, requests); the C CTAs of one (request, KV head) form a thread block
-// cluster and split that request's cached keys between them (split-KV).
+// cluster and split that request's cached keys between them (split-KV).  With sinks, a grid of several waves is a list of
+// clusters of two: whole contexts first, one per CTA, and a last wave of halves.
 // Decode CTA: 320 threads = eight arithmetic warps (two row groups of four: one warp per 32-key quarter of a tile,
 // a row group per four query rows), one MMA warp and one copying warp, two CTAs per SM; verify CTA: 576 threads =
 // sixteen arithmetic warps (four row groups of 16 rows) and the same two, one CTA per SM.  The two extra warps do
@@ -74,6 +75,7 @@ struct AttnArgs {
     const long long* cache_loc;
     const float* inv_freq;
     int B, Hq, Hkv, page_size, num_pages, window, sinks, nstages, longest_first;
+    int whole;  // > 0: clusters of two CTAs; so many (request, KV head) pairs, the first ones, have a CTA each, the others a cluster
     float qk_scale_factor, sm_scale, q_split_scale;
     int* status;
 };
@@ -157,8 +159,15 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     const int kq = warp & 3, rg = warp >> 2;  // 32-key quarter of the tile (= tensor-memory lane quarter), row group
     const int ktid = tid & 127;               // key inside the tile / channel d, depending on the phase
     const int r_lo = rg * NRG;                // this thread's query rows: [r_lo, r_lo + NRG)
-    const int C = gridDim.x, rank = blockIdx.x, h = blockIdx.y;
-    int b = blockIdx.z;
+    int C = gridDim.x, rank = blockIdx.x, h = blockIdx.y;  // chunks of this request, this CTA's
+    int b = blockIdx.z, home = 0;                          // home: the cluster's CTA that has chunk 0
+    if (SINKS && L == 1 && p.whole > 0) {
+        const int c = static_cast<int>(blockIdx.x) >> 1, r = static_cast<int>(blockIdx.x) & 1;
+        const bool alone = 2 * c < p.whole;
+        const int pair = alone ? 2 * c + r : c + p.whole / 2;
+        C = alone ? 1 : 2, rank = alone ? 0 : r, home = alone ? r : 0;
+        b = pair / p.Hkv, h = pair - b * p.Hkv;
+    }
     if (p.longest_first) {
         // More CTAs than the GPU holds at once, contexts of very different lengths: the CTAs are handed out in
         // grid order, so slice z takes the request with the z-th longest context (equal ones in their own order) and the
@@ -166,7 +175,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
         // z-th longest length bit by bit, counting over the CTA's threads, then the request that has it.  (Ranking all <= 256
         // lengths against one another took 3.4 us of each CTA's 55 at window 4096.)
         __shared__ int b_s;
-        const int z = blockIdx.z, i = threadIdx.x;
+        const int z = b, i = threadIdx.x;
         // (lengths that no request can have are brought into the range the bits cover)
         const int len = i < p.B ? min(max(p.seq_lens[i], 0), 2 * p.longest_first - 1) : -1;
         int v = 0;
@@ -725,14 +734,14 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     }
     csync();
     if (tid < NR) {
-        const int owner = tid / rows_per, nl = tid % rows_per;
+        const int owner = home + tid / rows_per, nl = tid % rows_per;
         const float lsum = (wred[0][tid] + wred[1][tid]) + (wred[2][tid] + wred[3][tid]);
         dsmem_st_f32(dsmem_addr(smem_u32(&mrg_m[rank * rows_per + nl]), owner), m_s[tid]);
         dsmem_st_f32(dsmem_addr(smem_u32(&mrg_l[rank * rows_per + nl]), owner), lsum);
     }
 #pragma unroll
     for (int n = 0; n < NRG; ++n) {
-        const int owner = (r_lo + n) / rows_per, nl = (r_lo + n) % rows_per;
+        const int owner = home + (r_lo + n) / rows_per, nl = (r_lo + n) % rows_per;
         dsmem_st_f32(dsmem_addr(s_mrg + ((rank * rows_per + nl) * 128 + ktid) * 4, owner), o_acc[n]);
     }
     }
@@ -872,6 +881,15 @@ int launch_attn(const MskAttnParams* q, int* status, cudaStream_t stream) {
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(C, q->Hkv, q->B);
+    // Under a window with sinks the contexts are alike, and a last wave that fills no more than half of the places reads at
+    // half the rate: its contexts are split in two (4 heads, window 4096 + 64: 256 requests 193 us, without 204 us; 96 requests 87 and
+    // 103; window 1024: 256 requests 94.5 and 96.5).
+    const int places = resident * 148, pairs = q->B * q->Hkv, rest = pairs % places;
+    if (SINKS && L == 1 && q->chunks == 0 && C == 1 && pairs > places && rest > 0 && 2 * rest <= places && tiles_max >= 2) {
+        a.whole = pairs - rest;
+        C = 2;
+        cfg.gridDim = dim3(a.whole + 2 * rest, 1, 1);
+    }
     cfg.blockDim = dim3(128 * RG + 64, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
