@@ -80,7 +80,9 @@ struct AttnArgs {
     int* status;
 };
 
-// cos and sin of this lane's two RoPE angles at a position.
+// cos and sin of this lane's two RoPE angles at a position.  The angle is the reference's product in 32 bits
+// (muse_attention_decode/reference.py:274); EXACT: its rounding error (up to 5e-4 at position 8192) is put back to first order.
+template <bool EXACT>
 __device__ __forceinline__ void rope_angles(const float* inv_freq, int pos, int lane, float (&c)[2], float (&s)[2]) {
     c[0] = c[1] = 1.0f, s[0] = s[1] = 0.0f;
     if (inv_freq != nullptr) {
@@ -89,6 +91,10 @@ __device__ __forceinline__ void rope_angles(const float* inv_freq, int pos, int 
         for (int h = 0; h < 2; ++h) {
             const float ang = fp * inv_freq[2 * lane + h];
             c[h] = cosf(ang), s[h] = sinf(ang);
+            if (EXACT) {
+                const float err = fmaf(fp, inv_freq[2 * lane + h], -ang), ch = c[h];
+                c[h] -= err * s[h], s[h] += err * ch;
+            }
         }
     }
 }
@@ -349,7 +355,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     // (decode: all rows and the new key turn by the same angles, which need nothing of the previous kernel)
     const bool turn = p.inv_freq != nullptr;
     float rc[2], rs[2];
-    if constexpr (L == 1) rope_angles(p.inv_freq, seq, lane, rc, rs);
+    if constexpr (L == 1) rope_angles<SINKS>(p.inv_freq, seq, lane, rc, rs);
     pdl_wait();
     const float k_scale = __ldg(p.k_scale), v_scale = __ldg(p.v_scale);
     const float qs = p.q_split_scale;
@@ -413,7 +419,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                 }
             }
         }
-        if constexpr (L != 1) rope_angles(p.inv_freq, seq + j, lane, rc, rs);
+        if constexpr (L != 1) rope_angles<SINKS>(p.inv_freq, seq + j, lane, rc, rs);
         norm_rope_row(x, p.qk_scale_factor, turn, rc, rs);
         if (L == 1 && tail_cta) {
             float dot = 0.0f;
@@ -660,7 +666,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
             const uint2 kr = *reinterpret_cast<const uint2*>(ksrc), vr = *reinterpret_cast<const uint2*>(vsrc);
             float kx[4] = {bf16lo(kr.x), bf16hi(kr.x), bf16lo(kr.y), bf16hi(kr.y)};
             const float vx[4] = {bf16lo(vr.x), bf16hi(vr.x), bf16lo(vr.y), bf16hi(vr.y)};
-            rope_angles(p.inv_freq, seq + j, lane, rc, rs);
+            rope_angles<SINKS>(p.inv_freq, seq + j, lane, rc, rs);
             norm_rope_row(kx, 1.0f, turn, rc, rs);
             uint32_t kb = 0, vb = 0;
 #pragma unroll
@@ -683,7 +689,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
             const size_t tok = static_cast<size_t>(b) * L + j;
             const uint2 raw = *reinterpret_cast<const uint2*>(p.qkv + tok * p.ld_qkv + (h * 8 + g) * 128 + 4 * lane);
             float x[4] = {bf16lo(raw.x), bf16hi(raw.x), bf16lo(raw.y), bf16hi(raw.y)};
-            rope_angles(p.inv_freq, seq + j, lane, rc, rs);
+            rope_angles<SINKS>(p.inv_freq, seq + j, lane, rc, rs);
             norm_rope_row(x, p.qk_scale_factor, turn, rc, rs);
             *reinterpret_cast<uint2*>(qf + n * 128 + 4 * lane) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         }
