@@ -21,6 +21,17 @@ def test_blocks_of_every_length(q_len, window, sinks):
     close(out, oattn.ref_stream(data, new_kv=(k_new, v_new))[0], f"{q_len} tokens")
 
 
+@pytest.mark.parametrize("batch,q_len", [(50, 8), (20, 40), (13, 2), (33, 3)])
+@pytest.mark.parametrize("page", [8, 128])
+def test_blocks_of_many_requests(batch, q_len, page):
+    """Blocks in more units than the GPU has SMs (the prep kernel lists them) and in fewer (every CTA finds its own), alone and
+    in pairs of CTAs."""
+    seqs = [(37 * i) % 311 for i in range(batch)]
+    data = streaming(oattn.make_input(batch, seqs, seed=batch, q_len=q_len, hq=32, hkv=4, page=page, window=60), 3)
+    out, k_new, v_new = run_step(data)
+    close(out, oattn.ref_stream(data, new_kv=(k_new, v_new))[0], f"{batch} x {q_len} tokens")
+
+
 def test_prompt_in_a_graph_with_fresh_inputs():
     """Captured once, replayed with new inputs in the same buffers: bit for bit the eager call; two graphs do not share
     memory."""
