@@ -3,7 +3,7 @@
 //
 //   prep     one CTA per token: RMSNorm, scale and RoPE of its queries (rounded to BF16, kept as FP16 in the workspace) and
 //            keys; keys and values quantised to E4M3 and written into the pages the page table names.  Keys and angles are
-//            taken in 64 bits (2 us of 310 at 4096 tokens).  One more CTA lists the work units (request, first token), unless
+//            taken in 64 bits (2 us of 310 for 16 prompts of 1 to 1024 tokens).  One more CTA lists the work units (request, first token), unless
 //            they are few and every CTA finds its own.  Bound by memory: 18 KB per token at 32 + 4 + 4 heads.
 //   main     one CTA, or a pair of CTAs on neighbouring SMs, per (unit of 32 or 64 new tokens, KV head, split): flash
 //            attention.  The 8 query heads of a KV head and the tokens together are the rows of the product: a CTA has 2
