@@ -448,7 +448,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // A new reference lies 2^kAhead above the row's maximum and serves until a score lies 2^kLazy above it:
                 // FP16 holds p up to 2^15, and what lies 2^-20 below the largest p may lose bits.
                 const float tops = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
-                const bool move = tops - m > kLazy;
+                // Rows behind the unit's last token (the next request's, or a padding row's leftovers) move nothing: the bits of
+                // a request are its own.
+                const bool move = live && tops - m > kLazy;
                 if (__any_sync(0xffffffffu, move)) {
                     // all of the warp's rows move up, not only those that must: four sinks first leave 32 low references, and
                     // one of the rows outgrew its own in most of the following steps
