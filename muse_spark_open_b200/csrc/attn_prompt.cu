@@ -10,15 +10,16 @@
 //            tiles of 128 rows = 16 tokens x 8 heads.
 //   combine  one warp per (token, head): joins the splits' (m, l, O); used when there are fewer units than SMs.
 //
-// Main kernel, per 128-key tile (FP16 tensor-core operands: E4M3 cache values and BF16 queries are exact in FP16, and
-// FP16 probabilities are off by 2^-12, so the result carries little more than its last rounding):
+// Main kernel, per 128-key tile (FP16 tensor-core operands: E4M3 cache values and BF16 queries are exact in FP16; FP16
+// probabilities are off by 2^-12 of their value down to 2^-22 of the row's largest, below that by 2^-33 of the largest, so the
+// result carries little more than its last rounding):
 //   copying warp     TMA boxes of the K and V pages into E4M3 staging
 //   converting warps E4M3 -> FP16 into the swizzled operand tiles, value rows no token sees as zeros
 //   MMA warp         S = Q K^T into TMEM (128 x 128 FP32 per row tile), O += P V with P from TMEM
 //   softmax warps    thread = row: the row's 128 scores come from TMEM in one go, no shuffles; p = 2^(s - m) goes back as
-//                    FP16 over the scores.  The running reference m is set ahead of the maximum and moves only when a score
-//                    outgrows what FP16 holds, so the accumulator in TMEM is rescaled once or twice per row, not per tile
-//                    (800 clocks each time, in whichever warp has such a row).
+//                    FP16 over the scores.  The running reference m lies below the maximum and moves only when a score
+//                    outgrows what FP16 holds, so the accumulator in TMEM is rescaled a few times per row, not per tile
+//                    (800 clocks each time and the wait for the last product, in whichever warp has such a row).
 // The products run ahead of the softmax in halves of 64 keys: while the softmax works on one half of a row tile's scores,
 // the tensor cores add the other half's product and put the next tile's scores in its place.  (With whole tiles each tile
 // waited 1300 clocks for its next scores, a third of the loop; a third row tile does not fit.)
@@ -68,8 +69,8 @@ struct Geo {
 static_assert(Geo<1>::kSmem <= 231000 && Geo<2>::kSmem <= 231000, "shared memory");
 constexpr float kNegRef = -1.0e30f;
 constexpr int kPolyEvery = 4;               // of the pairs of probabilities, every how manieth goes to the FMA pipe
-constexpr float kLazy = 15.0f;              // how far (in powers of two) a score may lie above its row's reference
-constexpr float kAhead = 4.0f;              // how far a new reference lies above the row's maximum
+constexpr float kLazy = 15.75f;             // how far (in powers of two) a score may lie above its row's reference
+constexpr float kBelow = 8.0f;              // how far a new reference lies below the row's maximum
 constexpr int kMaxUnitsHeader = 4;          // ints before the unit list: their number, padding
 constexpr int kBuckets = 256;
 
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
         const float scale = k_scale * p.s_scale;
         const int g_first = p_first + tok_of(g), g_last = g_first + kTok - 1;
-        float m = kNegRef, l = 0.0f;
+        float m = kNegRef, top = kNegRef, l = 0.0f;  // reference, maximum, sum
         bool ok = true;
         if ((g == 0 || two) && nt > 0) {
             for (int t = 0; t < 2 * nt; ++t) {  // 64 keys at a time
@@ -445,16 +446,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int e = 3; e < 15; e += 2) mx[c] = max3(mx[c], v(e), v(e + 1));
                     mx[c] = fmaxf(mx[c], v(15));
                 }
-                // A new reference lies 2^kAhead above the row's maximum and serves until a score lies 2^kLazy above it:
-                // FP16 holds p up to 2^15, and what lies 2^-20 below the largest p may lose bits.
+                // A new reference lies 2^kBelow below the row's maximum and serves until a score lies 2^kLazy above it.  So the
+                // row's largest p is 2^8 or more, and FP16's smallest step 2^-32 of it: thousands of keys may lie 2^-20 below
+                // one that draws the weight and still carry the output, when that one's value is small.  (References 2^4
+                // above the maximum lost such keys, 1.5 % of a row of 8192, and saved moves: 8192 tokens full 579 us against
+                // 607, three documents under a window 333 and 356.  Moving to the half tile's maximum instead of the row's:
+                // 635 and 359 us.)
                 const float tops = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
+                top = fmaxf(top, tops);
                 // Rows behind the unit's last token (the next request's, or a padding row's leftovers) move nothing: the bits of
                 // a request are its own.
                 const bool move = live && tops - m > kLazy;
                 if (__any_sync(0xffffffffu, move)) {
                     // all of the warp's rows move up, not only those that must: four sinks first leave 32 low references, and
                     // one of the rows outgrew its own in most of the following steps
-                    const float m_new = fmaxf(m, tops + kAhead);
+                    const float m_new = fmaxf(m, top - kBelow);
                     const float alpha = ex2(m - m_new);
                     m = m_new;
                     l *= alpha;
