@@ -62,8 +62,8 @@ def _scratch(pool: dict, q: bytes, shape, n: int):
     counts and are ordered anyway.  Lists longer than the pool has rows (and a first call inside a graph capture, whose memory
     is the graph's) get memory of their own, for the call."""
     kept = pool.get("scratch")
-    if kept is not None and (kept[0] != shape or kept[4] is not pool["refs"]):
-        kept = None  # a copy of another pool's dict, with counts of its own
+    if kept is not None and (kept[0] != shape or kept[4] is not pool["refs"] or kept[1] != kept[3].data_ptr()):
+        kept = None  # a copy of another pool, with counts of its own (a deep one: the address is still the other pool's)
     if kept is not None and n <= shape[0]:
         return kept[1], kept[2], None
     b = C.c_size_t()
