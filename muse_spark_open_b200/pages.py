@@ -23,6 +23,7 @@ The reference has no counterpart: its inputs come with a finished table (muse_at
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 
 import torch
@@ -83,7 +84,7 @@ def _caches(caches, pool: dict, index: int):
             raise abi.MskError("caches must be contiguous [num_pages, page_size, ...]")
         if c.get_device() != index:
             raise abi.MskError("the tensors of one call must be on one device")
-        bytes_ = c.stride(1) * c.element_size()
+        bytes_ = math.prod(shape[2:]) * c.element_size()  # not the stride: of an axis of length one it may be anything
         if token and bytes_ != token:
             raise abi.MskError("the caches of one call must have the same bytes per token")
         token = bytes_
