@@ -166,8 +166,8 @@ int msk_attn_prompt_scratch_bytes(const MskPromptParams* p, size_t* bytes);
  * every call can be captured.  `refs[p]` is the number of page-table entries that name page p; a page is free when it is 0.
  * New pages are the lowest free ones, given out in the order of the call's rows.  Calls on one pool are ordered by their
  * stream.  A row or page index out of range, a row that one call lists twice (extend, fork), a child that is also a parent,
- * new tokens that would go into a page which other rows share (seq_lens was set back behind a fork): MSK_ERR_BOUNDS in
- * `status`, and that entry is skipped.  No free page, or more tokens than max_pages hold:
+ * new tokens that would go into a page which other rows share (seq_lens was set back behind a fork), cu_seqlens that falls
+ * or passes `tokens` at an entry: MSK_ERR_BOUNDS in `status`, and that entry is skipped.  No free page, or more tokens than max_pages hold:
  * MSK_ERR_CAPACITY, and the positions concerned get no page (fork: the child is left empty).
  * The reference has no counterpart: its inputs come with a finished page table (muse_attention_decode/reference.py:168-253).
  */
@@ -183,7 +183,8 @@ typedef struct {
 int msk_pages_scratch_bytes(const MskPages* pool, int n, size_t* bytes);
 
 /* Room for new tokens: rows[j] gets pages for the positions seq_lens .. seq_lens + n_j - 1 that have none, n_j = q_len, or
- * cu_seqlens[j + 1] - cu_seqlens[j] when cu_seqlens is given (then `tokens` is the length of cache_loc).  seq_lens stays.
+ * cu_seqlens[j + 1] - cu_seqlens[j] when cu_seqlens is given (then `tokens`, at least its last entry, is the length of
+ * cache_loc).  seq_lens stays.
  * cache_loc (int64, or NULL): the flat cache row of each new token, -1 where there is none; entries behind the last row's
  * tokens are left as they were. */
 int msk_pages_extend(const MskPages* pool, const int32_t* rows, int n, int q_len, const int32_t* cu_seqlens, int tokens,

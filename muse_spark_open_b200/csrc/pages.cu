@@ -143,15 +143,16 @@ __device__ __forceinline__ int slice_total(const int* counts, int gwarp, int nwa
     return warp_total(all);
 }
 
-// The new tokens of list entry j: [first logical page, last] of row; tokens.
-__device__ __forceinline__ void span_of(const PlanArgs& p, int row, int j, int* seq, int* n_tok, int* first_loc) {
-    *seq = p.seq_lens[row];
-    if (p.cu != nullptr) {
-        const int a = min(max(p.cu[j], 0), p.tokens), b = min(max(p.cu[j + 1], 0), p.tokens);
-        *first_loc = a, *n_tok = max(b - a, 0);
-    } else {
+// The new tokens of list entry j: how many, and where they begin in cache_loc; false where cu_seqlens falls or names more
+// tokens than there are (then those that cache_loc has).
+__device__ __forceinline__ bool tokens_of(const PlanArgs& p, int j, int* n_tok, int* first_loc) {
+    if (p.cu == nullptr) {
         *first_loc = j * p.q_len, *n_tok = p.q_len;
+        return true;
     }
+    const int a = p.cu[j], b = p.cu[j + 1];
+    *first_loc = min(max(a, 0), p.tokens), *n_tok = max(min(max(b, 0), p.tokens) - *first_loc, 0);
+    return 0 <= a && a <= b && b <= p.tokens;
 }
 
 // A page that new tokens of a row must not go into: another row holds it too, or there is no such page.
@@ -239,9 +240,13 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
             bool ok = row >= 0 && row < p.rows && __ldcg(p.claim + row) == j;
             int need = 0;
             if (!ok && lane == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 2, row, j);
+            int n_tok, first_loc;
+            if (!tokens_of(p, j, &n_tok, &first_loc)) {
+                if (lane == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 8, p.cu[j + 1], p.tokens);
+                ok = false;
+            }
             if (ok) {
-                int seq, n_tok, first_loc;
-                span_of(p, row, j, &seq, &n_tok, &first_loc);
+                const int seq = p.seq_lens[row];
                 ok = seq >= 0;
                 const int first = seq >> p.page_log;
                 const int last = n_tok > 0 ? static_cast<int>((static_cast<long long>(seq) + n_tok - 1) >> p.page_log) : first - 1;
@@ -331,10 +336,9 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
     if constexpr (!kFork) {
         for (int j = gwarp; j < p.n; j += kAllWarps) {
             const int need = __ldcg(p.need + j), off = __ldcg(p.offs + j), row = p.list[j];
-            int seq = 0, n_tok = 0, first_loc = 0;
-            if (row >= 0 && row < p.rows) span_of(p, row, j, &seq, &n_tok, &first_loc);
-            else if (p.cu == nullptr) first_loc = j * p.q_len, n_tok = p.q_len;
-            else first_loc = min(max(p.cu[j], 0), p.tokens), n_tok = max(min(max(p.cu[j + 1], 0), p.tokens) - first_loc, 0);
+            int n_tok, first_loc;
+            tokens_of(p, j, &n_tok, &first_loc);
+            const int seq = need >= 0 ? p.seq_lens[row] : 0;
             int* held = need >= 0 ? p.page_table + static_cast<size_t>(row) * p.max_pages : nullptr;
             if (need > 0) {
                 const int first = seq >> p.page_log;

@@ -16,7 +16,7 @@ Everything happens on the device, in place and in stream order (order the stream
 nothing is read back, so all calls can be captured in a CUDA
 graph.  New pages are the lowest free ones, given out in the order of the rows: results do not depend on scheduling.
 Problems with the contents (a row out of range or listed twice, no free page, seq_lens set back into pages that a fork shares
-and then extended) are reported in the status word
+and then extended, cu_seqlens that falls or names more tokens than `tokens`) are reported in the status word
 (`abi.status_for(device).raise_if_set()`), and the entries concerned are skipped; include/msk.h says how.
 The reference has no counterpart: its inputs come with a finished table (muse_attention_decode/reference.py:168-253).
 """
@@ -92,15 +92,19 @@ def _caches(caches, pool: dict, index: int):
     return struct.pack(f"{len(ptrs)}P", *ptrs), len(ptrs), token or 16
 
 
-def extend(pool: dict, rows: torch.Tensor, q_len: int = 1, cu_seqlens: torch.Tensor | None = None, tokens: int = 0) -> torch.Tensor:
-    """Pages for the next `q_len` tokens of each row, or for cu_seqlens[j + 1] - cu_seqlens[j] of row j (then `tokens` rows
-    in all, padding included).  Returns cache_loc int64 [len(rows) * q_len] (or [tokens]): the flat cache row of each new
+def extend(pool: dict, rows: torch.Tensor, q_len: int = 1, cu_seqlens: torch.Tensor | None = None,
+           tokens: int | None = None) -> torch.Tensor:
+    """Pages for the next `q_len` tokens of each row, or for cu_seqlens[j + 1] - cu_seqlens[j] of row j (then `tokens`, which
+    has to be given, rows in all, padding included).  Returns cache_loc int64 [len(rows) * q_len] (or [tokens]): the flat cache row of each new
     token, -1 where there is none.  seq_lens stays: the caller advances it when the tokens are in."""
     n = rows.shape[0]
     if cu_seqlens is None:
+        tokens = 0
         q, shape, index = _args(pool, rows)
         loc, cu = torch.empty(n * q_len, dtype=torch.int64, device=rows.device), 0
     else:
+        if tokens is None or tokens < 0:
+            raise abi.MskError("with cu_seqlens, tokens (its last entry or more) has to be given")
         q, shape, index = _args(pool, rows, cu_seqlens)
         if cu_seqlens.shape[0] != n + 1:
             raise abi.MskError("cu_seqlens must have one entry more than rows")

@@ -1,0 +1,30 @@
+"""What the page calls find wrong in their lists is reported, and the entries concerned are skipped."""
+import pytest
+import torch
+
+from oracle.pages import Pool
+from test_gpu_pages import i32, same, status, upload
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("num_pages", [50, 20000])  # one CTA plans, or a cluster
+@pytest.mark.parametrize("cu,tokens,bad", [([0, 5, 25, 30], 24, [1, 2]), ([0, 5, 25, 30], 29, [2]), ([0, 5, 25, 30], 0, [0, 1, 2]), ([0, 9, 5, 5], 9, [1]),
+                                           ([-3, 2, 4, 6], 6, [0]), ([0, 3, 3, 2 ** 31 - 1], 3, [2])])
+def test_ragged_extend_reports_tokens_that_have_no_entry(num_pages, cu, tokens, bad):
+    from muse_spark_open_b200 import pages
+    model = Pool(num_pages, 4, 5, 12)
+    for row, n in enumerate([3, 0, 8, 1]):
+        model.extend([row], [n])
+        model.seq[row] = n
+    pool, _, _ = upload(model, [])
+    rows = [2, 0, 3]
+    loc = pages.extend(pool, i32(rows), cu_seqlens=i32(cu), tokens=tokens)
+    assert status() == {"bounds"}
+    want = [-1] * tokens
+    for j in range(3):
+        if j not in bad:
+            want[cu[j]:cu[j + 1]] = model.extend([rows[j]], [cu[j + 1] - cu[j]])[0]
+    assert loc.tolist() == want
+    same(model, pool)
+    assert model.consistent()

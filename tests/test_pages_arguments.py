@@ -50,3 +50,10 @@ def test_caches_of_other_layouts_are_refused():
                 torch.empty((6, 2, 4, 16), dtype=torch.uint8).transpose(1, 2), torch.empty((6, 4, 2, 16), dtype=torch.int16)):
         with pytest.raises(abi.MskError):
             pages._caches([good, bad], pool, -1)
+
+
+@pytest.mark.parametrize("more", [{}, {"tokens": None}, {"tokens": -1}])
+def test_ragged_extend_wants_to_know_how_many_tokens(more):
+    pool = pages.prepare(8, 4, 2, 3, device="cpu")
+    with pytest.raises(abi.MskError, match="tokens"):
+        pages.extend(pool, torch.zeros(1, dtype=torch.int32), cu_seqlens=torch.tensor([0, 3], dtype=torch.int32), **more)
