@@ -167,8 +167,9 @@ int msk_attn_prompt_scratch_bytes(const MskPromptParams* p, size_t* bytes);
  * New pages are the lowest free ones, given out in the order of the call's rows.  Calls on one pool are ordered by their
  * stream.  A row or page index out of range, a row that one call lists twice (extend, fork), a child that is also a parent,
  * new tokens that would go into a page which other rows share (seq_lens was set back behind a fork), cu_seqlens that falls
- * or passes `tokens` at an entry: MSK_ERR_BOUNDS in `status`, and that entry is skipped.  No free page, or more tokens than max_pages hold:
- * MSK_ERR_CAPACITY, and the positions concerned get no page (fork: the child is left empty).
+ * or passes `tokens` at an entry, a row (extend) or parent (fork) whose seq_lens is negative: MSK_ERR_BOUNDS in `status`, and
+ * that entry is skipped.  No free page, or more tokens than max_pages hold: MSK_ERR_CAPACITY, and the positions concerned get
+ * no page (fork: the child is left empty).
  * The reference has no counterpart: its inputs come with a finished page table (muse_attention_decode/reference.py:168-253).
  */
 typedef struct {

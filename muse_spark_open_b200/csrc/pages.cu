@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
                 ok = ok && par >= 0 && par < p.rows && __ldcg(p.is_parent + row) == 0;
                 int4 op = make_int4(-1, -1, 0, 0);
                 if (ok) {
-                    const int seq = max(p.seq_lens[par], 0), full = seq >> p.page_log, part = seq & (p.page_size - 1);
-                    if (full + (part > 0) <= p.max_pages) {
+                    const int seq = p.seq_lens[par], full = seq >> p.page_log, part = seq & (p.page_size - 1);
+                    if (seq >= 0 && full + (part > 0) <= p.max_pages) {
                         op.w = 1;
                         if (part > 0) {
                             op.x = p.page_table[static_cast<size_t>(par) * p.max_pages + full];
@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
             } else if (ok) {
                 const int seq = p.seq_lens[row];
                 ok = seq >= 0;
+                if (!ok) report(p.status, MSK_ERR_BOUNDS, kWhere | 9, seq, row);
                 const int last = static_cast<int>((static_cast<long long>(seq) + p.q_len - 1) >> p.page_log);
                 if (ok && p.q_len > 0 && last >= p.max_pages) report(p.status, MSK_ERR_CAPACITY, kWhere | 3, last, p.max_pages);
                 if (ok && p.q_len > 0)
@@ -248,6 +249,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
             if (ok) {
                 const int seq = p.seq_lens[row];
                 ok = seq >= 0;
+                if (!ok && lane == 0) report(p.status, MSK_ERR_BOUNDS, kWhere | 9, seq, row);
                 const int first = seq >> p.page_log;
                 const int last = n_tok > 0 ? static_cast<int>((static_cast<long long>(seq) + n_tok - 1) >> p.page_log) : first - 1;
                 if (ok && last >= p.max_pages && lane == 0) report(p.status, MSK_ERR_CAPACITY, kWhere | 3, last, p.max_pages);
@@ -423,7 +425,7 @@ __global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(PlanArgs p, Ca
         const int4 op = __ldcg(p.ops + j);
         if (op.w == 0) return;
         const int child = p.list[j], par = p.parents[j];
-        const int seq = max(p.seq_lens[par], 0), full = seq >> p.page_log;
+        const int seq = p.seq_lens[par], full = seq >> p.page_log;
         for (int lp = part * kCopyThreads + static_cast<int>(threadIdx.x); lp < p.max_pages; lp += blocks_per_row * kCopyThreads) {
             int* e = p.page_table + static_cast<size_t>(child) * p.max_pages + lp;
             const int old = *e;

@@ -16,8 +16,8 @@ Everything happens on the device, in place and in stream order (order the stream
 nothing is read back, so all calls can be captured in a CUDA
 graph.  New pages are the lowest free ones, given out in the order of the rows: results do not depend on scheduling.
 Problems with the contents (a row out of range or listed twice, no free page, seq_lens set back into pages that a fork shares
-and then extended, cu_seqlens that falls or names more tokens than `tokens`) are reported in the status word
-(`abi.status_for(device).raise_if_set()`), and the entries concerned are skipped; include/msk.h says how.
+and then extended, cu_seqlens that falls or names more tokens than `tokens`, negative seq_lens) are reported in the status
+word (`abi.status_for(device).raise_if_set()`), and the entries concerned are skipped; include/msk.h says how.
 The reference has no counterpart: its inputs come with a finished table (muse_attention_decode/reference.py:168-253).
 """
 from __future__ import annotations
