@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(PlanArgs p) {
                         if (part > 0) {
                             op.x = p.page_table[static_cast<size_t>(par) * p.max_pages + full];
                             op.z = part;
+                            if (op.x >= p.num_pages) report(p.status, MSK_ERR_BOUNDS, kWhere | 6, op.x, p.num_pages);
                             if (op.x >= p.num_pages || op.x < 0) op.x = -1;
                             need = op.x >= 0;
                         }
@@ -431,8 +432,12 @@ __global__ void __launch_bounds__(kCopyThreads) pages_fork_kernel(PlanArgs p, Ca
             const int old = *e;
             int id = -1;
             if (op.w == 1) id = lp < full ? p.page_table[static_cast<size_t>(par) * p.max_pages + lp] : lp == full ? op.y : -1;
+            if (id >= p.num_pages) {
+                report(p.status, MSK_ERR_BOUNDS, kWhere | 6, id, p.num_pages);
+                id = -1;
+            }
             *e = id;
-            if (id >= 0 && id < p.num_pages && lp < full) atomicAdd(p.refs + id, 1);
+            if (id >= 0 && lp < full) atomicAdd(p.refs + id, 1);
             if (old >= 0 && old < p.num_pages) atomicSub(p.refs + old, 1);  // what the child's row held before
         }
         if (part == 0 && threadIdx.x == 0) p.seq_lens[child] = op.w == 1 ? seq : 0;

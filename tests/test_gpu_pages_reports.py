@@ -63,3 +63,22 @@ def test_fork_reports_a_parent_of_negative_length(seq):
     assert not model.fork([0], [3], caches)
     pool["seq_lens"][1] = 5
     same(model, pool, caches, dev)
+
+
+@pytest.mark.parametrize("at", [0, 1])  # a page that is shared, and the last one, which is copied
+def test_fork_reports_a_page_that_does_not_exist(at):
+    """The child gets no page there, the rest of the fork goes through."""
+    from muse_spark_open_b200 import pages
+    model = Pool(30, 4, 5, 6)
+    for row, n in enumerate([7, 5]):
+        model.extend([row], [n])
+        model.seq[row] = n
+    model.refs[model.table[0][at]] = 0
+    model.table[0][at] = -1
+    pool, caches, dev = upload(model, [(1, 16)])
+    pool["page_table"][0, at] = 10 ** 6
+    pages.fork(pool, i32([0, 1]), i32([2, 3]), dev)
+    assert status() == {"bounds"}
+    assert not model.fork([0, 1], [2, 3], caches)
+    pool["page_table"][0, at] = -1
+    same(model, pool, caches, dev)
