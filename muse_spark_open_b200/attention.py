@@ -5,7 +5,7 @@ muse_attention_decode/submission.py:37-65; the new tokens' K/V are written into
 `data["k_cache"]` / `data["v_cache"]` in place at `data["cache_loc"]`, like the reference.
 With a window, `config["sinks"]` (default 0) first positions stay visible to every token.
 q_len is 1 (decode) or 8 (verify) as in the reference, or any other length: blocks other than 1 and 8, and blocks of 8 with
-sinks, write the new rows where the page table says (cache_loc says the same in the reference, submission.py:37-65).
+a window and sinks, write the new rows where the page table says (cache_loc says the same in the reference, submission.py:37-65).
 Nothing derived from `data` is cached between calls; only the RoPE frequency table (a function of
 theta and head_dim) is kept per device.
 """
@@ -72,7 +72,7 @@ def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
         flat = qkv.view(b * l, -1)
         cols, ld = flat.shape[1] if flat.stride(1) == 1 else 0, flat.stride(0)
     out = torch.empty((b, l, wide), dtype=torch.bfloat16, device=qkv.device)
-    if l != 1 and (l != 8 or cfg.get("sinks", 0)) and not chunks and not stages:
+    if l != 1 and (l != 8 or (cfg["window"] and cfg.get("sinks", 0))) and not chunks and not stages:
         # blocks of other lengths, and verify blocks with sinks: the prompt kernels (16 requests x 8 tokens, window 1024 + 4
         # sinks: 21 us against 51 us for the verify kernel, whose results without sinks stay what they were)
         _run_prompt(data, cfg, qkv, b * l, cols, ld, out, wide, None, l, 0)
