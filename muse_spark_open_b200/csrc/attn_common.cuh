@@ -82,5 +82,9 @@ __device__ __forceinline__ uint32_t f_to_e4m3(float a) {
 __device__ __forceinline__ uint32_t f_to_e5m2(float a) {
     return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E5M2);
 }
+__device__ __forceinline__ bool has_nan(uint4 v) {  // one of 16 E4M3 values is NaN (0x7f with either sign)
+    const uint32_t k = 0x7f7f7f7fu, one = 0x01010101u;
+    return ((((v.x & k) + one) | ((v.y & k) + one) | ((v.z & k) + one) | ((v.w & k) + one)) & 0x80808080u) != 0;
+}
 
 }  // namespace msk

@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[4 * kAttnMaxStages + 2];
     __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t spoilt;  // verify: one bit per token of the block that sees a NaN value which others do not see
     __shared__ int page_ids[kPageIds];
     __shared__ __align__(16) float wred_s[PBUF][4][NR];  // per-warp maxima of a tile (alternating buffers)
     auto& wred = wred_s[0];
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
         for (int s = 0; s < nst; ++s) mbar_init(full(s), 1), mbar_init(full_v(s), 1), mbar_init(sdone(s), 1), mbar_init(odone(s), 1);
         mbar_init(pready(0), NWARP_C);
         mbar_init(pready(1), NWARP_C);
+        spoilt = 0;
         fence_mbar_init();
     }
     const int seq = p.seq_lens[b];
@@ -597,12 +599,21 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                 }
             }
             // V rows that no query row sees -- past the cached length, or between the sinks and the window -- may hold
-            // anything (even NaN bytes): zero them so that 0 * V stays 0
-            if (rg == 0 && (pos >= seq || (W > 0 && pos <= seq - W && !sink))) {
+            // anything (even NaN bytes): zero them so that 0 * V stays 0.  So must those that hold a NaN and that only the
+            // block's first tokens see, the window leaving them inside the block; those tokens are noted.
+            if (rg == 0 && (pos >= seq || (W > 0 && pos <= seq - W + (L - 1) && !sink))) {
                 ok = mbar_wait(full_v(slot), ph, p.status, where | 12) && ok;
                 uint8_t* vrow = gbase + slot * kStageBytes + kTileKeys * 128 + ktid * 128;
+                bool zero = L == 1 || pos >= seq || pos <= seq - W;
+                if (!zero) {
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) zero = has_nan(reinterpret_cast<const uint4*>(vrow)[c]) || zero;
+                    if (zero) atomicOr(&spoilt, (1u << (pos - seq + W)) - 1u);  // tokens [0, pos - (seq - W))
+                }
+                if (zero) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(vrow)[c] = make_uint4(0, 0, 0, 0);
+                    for (int c = 0; c < 8; ++c) reinterpret_cast<uint4*>(vrow)[c] = make_uint4(0, 0, 0, 0);
+                }
             }
             if constexpr (L != 1) rg_sync();
             // p = 2^(s - m) as two E4M3 terms into P buffer i & 1 (its previous reader, the second MMA of tile
@@ -677,6 +688,12 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                 knew[j * 128 + 4 * lane + i] = e4m3_to_f(a);
                 vnew[j * 128 + 4 * lane + i] = e4m3_to_f(c);
             }
+            if (__any_sync(0xffffffffu, has_nan(make_uint4(vb, 0, 0, 0)))) {  // zeros, and a note to the tokens that see it
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vnew[j * 128 + 4 * lane + i] = 0.0f;
+                const int to = W > 0 && !(SINKS && seq + j < snk) ? min(L - j, W) + j : L;
+                if (lane == 0) atomicOr(&spoilt, (1u << to) - (1u << j));
+            }
             if (row_ok) {
                 const size_t off = (static_cast<size_t>(row) * p.Hkv + h) * 128 + 4 * lane;
                 *reinterpret_cast<uint32_t*>(p.k_cache + off) = kb;
@@ -724,7 +741,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
 #pragma unroll
             for (int r = 0; r < L; ++r) {
                 const float sc = sc_tail[r_lo + n][r];
-                const float pr = sc > 0.5f * kNeg ? ex2(sc - m) : 0.0f;
+                const float pr = ex2(sc - m);  // 0 where the row does not see the token, NaN where a score is
                 o += pr * kPScale * (L == 1 ? vnew_d : vnew[r * 128 + ktid]);
                 if (ktid == r) l_part[n] += pr;
             }
@@ -741,7 +758,8 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     csync();
     if (tid < NR) {
         const int owner = home + tid / rows_per, nl = tid % rows_per;
-        const float lsum = (wred[0][tid] + wred[1][tid]) + (wred[2][tid] + wred[3][tid]);
+        float lsum = (wred[0][tid] + wred[1][tid]) + (wred[2][tid] + wred[3][tid]);
+        if (L != 1 && (spoilt >> (tid >> 3) & 1)) lsum = __int_as_float(0x7fffffff);  // its token sees a NaN value
         dsmem_st_f32(dsmem_addr(smem_u32(&mrg_m[rank * rows_per + nl]), owner), m_s[tid]);
         dsmem_st_f32(dsmem_addr(smem_u32(&mrg_l[rank * rows_per + nl]), owner), lsum);
     }
@@ -768,7 +786,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
             lsum += wgt * mrg_l[src * rows_per + nl];
             o += wgt * mrg_o[(src * rows_per + nl) * 128 + ktid];
         }
-        const float vv = lsum > 0.0f ? o * (v_scale / kPScale) / lsum : 0.0f;
+        const float vv = lsum != 0.0f ? o * (v_scale / kPScale) / lsum : 0.0f;  // NaN stays NaN
         val[k] = vv;
         const float ss = warp_sum(vv * vv);
         if (lane == 0) wred[kq][nl] = ss;

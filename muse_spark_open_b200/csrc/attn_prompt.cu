@@ -286,10 +286,6 @@ __global__ void __launch_bounds__(256) prompt_prep_kernel(PromptArgs p) {
 __device__ __forceinline__ uint32_t low_bits(int n) {  // bits [0, n) set, n clamped to [0, 32]
     return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
-__device__ __forceinline__ bool has_nan(uint4 v) {  // one of 16 E4M3 values is NaN (0x7f with either sign)
-    const uint32_t k = 0x7f7f7f7fu, one = 0x01010101u;
-    return ((((v.x & k) + one) | ((v.y & k) + one) | ((v.z & k) + one) | ((v.w & k) + one)) & 0x80808080u) != 0;
-}
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
