@@ -59,6 +59,8 @@ constexpr int kMaxTilesPerCta = 160;
 constexpr int kPageIds = 2 * kMaxTilesPerCta;  // page ids a CTA keeps in shared memory: every tile's with pages of 64 and more
 constexpr float kNeg = -1.0e30f;
 constexpr float kPScale = 256.0f;  // p in [0, 1] is stored as p * 256 (E4M3 / E5M2 range)
+// With sinks, how far (in powers of two) a tile's reference may lie below the row's maximum so far.
+constexpr float kFar = 40.0f;
 
 struct AttnArgs {
     const __nv_bfloat16* qkv;
@@ -160,6 +162,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     __shared__ __align__(16) float wred_s[PBUF][4][NR];  // per-warp maxima of a tile (alternating buffers)
     auto& wred = wred_s[0];
     __shared__ float m_s[NR], alpha_s[PBUF][NR], mrg_m[NR], mrg_l[NR];
+    __shared__ float top_s[SINKS && L != 1 ? NR : 1];  // the rows' maxima, where those are not the references
     __shared__ float sc_tail[NR][L];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -297,6 +300,7 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     for (int i = tid; i < (1 + PBUF) * QP_BYTES / 16 && tid < NTHR_F; i += NTHR_F)
         reinterpret_cast<uint4*>(g_q)[i] = make_uint4(0, 0, 0, 0);
     if (tid < NR) m_s[tid] = kNeg;
+    if (SINKS && L != 1 && tid < NR) top_s[tid] = kNeg;
     tc_fence_before();
     // barrier 5: the table and the zeroed operands exist (the copying warp waits for this one, the others only
     // arrive); barrier 4: the mbarriers and the tensor-memory address exist (the other way round)
@@ -454,8 +458,19 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
     bool ok = true;
     // decode keeps the running maxima and the rescale factors replicated in every thread's registers
     float m_r[L == 1 ? NRG : 1], alpha_r[L == 1 ? NRG : 1];  // of rows r_lo + g
+    float top_r[L == 1 && SINKS ? NRG : 1];                  // their maxima, where those are not the references
 #pragma unroll
     for (int g = 0; g < (L == 1 ? NRG : 1); ++g) m_r[g] = kNeg, alpha_r[g] = 1.0f;
+#pragma unroll
+    for (int g = 0; g < (L == 1 && SINKS ? NRG : 1); ++g) top_r[g] = kNeg;
+    // The reference of a tile's probabilities.  A first token that stays visible often draws most of a row's weight and has
+    // a small value: the window's keys carry the output although they lie 2^-20 and more below it, where two E4M3 terms end
+    // (4096 keys 2^-23 below it: single tokens were off by 0.9 % of a row, blocks of 8 by 4 %).  So with sinks a tile's
+    // reference is its own maximum, and the running sums follow it up and down.
+    auto reference = [&](float tile, float& top) {
+        top = fmaxf(top, tile);
+        return fmaxf(tile, top - kFar);
+    };
 
     // scores of BR query rows (c0 .. c0+BR-1) for this thread's key: both split terms
     auto load_scores = [&](int i, int c0, float (&sc)[BR]) {
@@ -584,7 +599,9 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                 }
 #pragma unroll
                 for (int g = 0; g < NRG; ++g) {
-                    const float mn = fmaxf(tm[g], m_r[g]);
+                    float mn;
+                    if constexpr (SINKS) mn = reference(tm[g], top_r[g]);
+                    else mn = fmaxf(tm[g], m_r[g]);
                     alpha_p[g] = alpha_r[g];
                     alpha_r[g] = ex2(m_r[g] - mn);
                     m_r[g] = mn;
@@ -593,7 +610,10 @@ __global__ void __launch_bounds__(128 * RG + 64, (L == 1 && RG <= 2) ? 2 : 1)
                 if (ktid < NRG) {
                     const int r = r_lo + ktid;
                     const float mo = m_s[r];
-                    const float mn = fmaxf(fmaxf(fmaxf(wred_s[i & 1][0][r], wred_s[i & 1][1][r]), fmaxf(wred_s[i & 1][2][r], wred_s[i & 1][3][r])), mo);
+                    const float tile = fmaxf(fmaxf(wred_s[i & 1][0][r], wred_s[i & 1][1][r]), fmaxf(wred_s[i & 1][2][r], wred_s[i & 1][3][r]));
+                    float mn;
+                    if constexpr (SINKS) mn = reference(tile, top_s[r]);
+                    else mn = fmaxf(tile, mo);
                     alpha_s[i & 1][r] = ex2(mo - mn);
                     m_s[r] = mn;
                 }

@@ -84,3 +84,20 @@ def test_prompt_with_a_first_token_that_stays_visible():
         abi.status_for("cuda").raise_if_set("attention")
         row, element = off(out, data)
         assert row < 3e-3 and element < 2e-3, (new, row, element)
+
+
+@pytest.mark.parametrize("nats", [12.0, 16.0, 20.0])
+@pytest.mark.parametrize("sinks", [4, 64, 300])
+@pytest.mark.parametrize("q_len,chunks", [(1, 0), (1, 1), (8, 1), (8, 2)])
+def test_steps_with_a_first_token_that_stays_visible(q_len, chunks, sinks, nats):
+    """Single tokens and blocks on the verify kernel.  Their probabilities are two E4M3 terms, off by 2^-8 of their value at most and
+    independently, so by nothing over thousands of keys, down to 2^-22 of the tile's largest.  Keys in the tile of key 0 may be
+    lost: at most 127 of 4400, which carry at most a tenth of the output where they are (from 15 nats on), so 3e-3 of a row;
+    with the rounding to BF16 5e-3.  An element of 0.7 may miss as much of itself, 3.5e-3, and that rounding."""
+    from muse_spark_open_b200 import abi, attention
+    data = far_weights([9000, 6000], q_len, 6, window=4096, sinks=sinks, nats=nats)
+    out = attention.kernel_fn(oattn.to_device(data, "cuda"), chunks=chunks)
+    torch.cuda.synchronize()
+    abi.status_for("cuda").raise_if_set("attention")
+    row, element = off(out, data)
+    assert row < 5e-3 and element < 3.5e-3, (row, element)
