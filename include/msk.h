@@ -91,6 +91,7 @@ int msk_proj_scratch_bytes(int M, int N, int K, int splits, int token_splits, si
  * Stands in for muse_attention_decode/submission.py `kernel_fn` (:2363-2372) and the kernels behind it
  * (`attnc_kernel` :1604-1856, `attnpcc_kernel` :1915-2284, `attn_kernel` + `_prep` + `_attn_combine`
  * :293-539,115-173); the fields mirror its `Inputs` / `Config` (:37-65).
+ * RoPE turns by the reference's product of position and frequency in 32 bits, with sinks by the exact one.
  * Built for head_dim 128, Hq = 8 * Hkv, page_size a power of two in [8, 128].
  */
 typedef struct {
@@ -129,6 +130,7 @@ int msk_attn_decode(const MskAttnParams* p, int* status, void* stream);
  * is reported in `status` and not written.  Reads of a page-table entry of -1 below the window and above the sinks never
  * happen.  Stands beside msk_attn_decode, whose counterpart in the reference has only 1 or 8 new tokens per request
  * (muse_attention_decode/submission.py:2363-2372).
+ * RoPE turns by the exact angle.
  * Built for head_dim 128, Hq = 8 * Hkv, page_size a power of two in [8, 128], sm_scale > 0.
  */
 typedef struct {

@@ -6,6 +6,10 @@ muse_attention_decode/submission.py:37-65; the new tokens' K/V are written into
 With a window, `config["sinks"]` (default 0) first positions stay visible to every token.
 q_len is 1 (decode) or 8 (verify) as in the reference, or any other length: blocks other than 1 and 8, and blocks of 8 with
 a window and sinks, write the new rows where the page table says (cache_loc says the same in the reference, submission.py:37-65).
+RoPE's angle is the reference's product in 32 bits for tokens and blocks of 8 without sinks, off by up to 2^-11 rad at positions
+8192 to 16384 and twice that at twice the position; prompts, other blocks and steps with sinks turn by the exact one.  They may
+share a cache: each key has its own token's angle either way, and the two differ by less than the queries' other roundings move
+a score.
 Nothing derived from `data` is cached between calls; only the RoPE frequency table (a function of
 theta and head_dim) is kept per device.
 """
