@@ -127,7 +127,8 @@ int msk_attn_decode(const MskAttnParams* p, int* status, void* stream);
  * quantised and written into the pages the page table names for those positions, and attended from there.  Tokens see the
  * positions up to their own inside the window, and the first `sinks` ones.  Requests may bring no token; rows of qkv / out
  * outside every request do not matter and stay as they are.  A new token whose position has no page (-1, or beyond max_pages)
- * is reported in `status` and not written.  Reads of a page-table entry of -1 below the window and above the sinks never
+ * is reported in `status` and not written.  cu_seqlens_q that falls, is negative or passes T is reported too; the requests
+ * it concerns are cut to the rows there are.  Reads of a page-table entry of -1 below the window and above the sinks never
  * happen.  Stands beside msk_attn_decode, whose counterpart in the reference has only 1 or 8 new tokens per request
  * (muse_attention_decode/submission.py:2363-2372).
  * RoPE turns by the exact angle.

@@ -50,7 +50,7 @@ namespace {
 
 constexpr int kTile = 128;                  // keys per tile
 constexpr int kTok = 16;                    // tokens per row tile
-constexpr int kThreads = 512;               // softmax A | softmax B | converting | MMA, copying, one that waits for the queries, one idle
+constexpr int kThreads = 512;               // softmax A | softmax B | converting | MMA, copying, one that waits for the queries, one that checks the lists
 constexpr int kQBytes = 32768;              // one row tile of queries: two swizzled halves of 64 channels
 template <int CG>
 struct Geo {
@@ -794,6 +794,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ================ this CTA's queries have arrived: tell the MMA warp
             const bool ok = mbar_wait(q_here, 0, p.status, where | 15);
             if (lane == 0 && ok) arrive_issuer(q_full);
+            __syncwarp();
+        } else if (warp == 15 && blockIdx.x == 0 && p.cu != nullptr) {
+            // ================ the spare warp of the first CTA: requests that name rows which are not there
+            for (int r = lane; r < p.B; r += 32) {
+                const int from = p.cu[r], to = p.cu[r + 1];
+                if (from < 0 || to < from || to > p.T) report(p.status, MSK_ERR_BOUNDS, where | 16, to, p.T);
+            }
             __syncwarp();
         }
     }
