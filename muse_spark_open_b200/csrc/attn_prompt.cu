@@ -70,7 +70,8 @@ static_assert(Geo<1>::kSmem <= 231000 && Geo<2>::kSmem <= 231000, "shared memory
 constexpr float kNegRef = -1.0e30f;
 constexpr int kPolyEvery = 4;               // of the pairs of probabilities, every how manieth goes to the FMA pipe
 constexpr float kLazy = 15.75f;             // how far (in powers of two) a score may lie above its row's reference
-constexpr float kBelow = 8.0f;              // how far a new reference lies below the row's maximum
+constexpr float kBelow = 2.0f;              // how far a new reference lies below the row's maximum: this and log2 of the key tiles,
+constexpr float kMostBelow = 13.0f;         // at most this
 constexpr int kMaxUnitsHeader = 4;          // ints before the unit list: their number, padding
 constexpr int kBuckets = 256;
 
@@ -408,6 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t t_s = tmem + lanes + g * 128, t_o = tmem + lanes + 256 + g * 128;
         const float scale = k_scale * p.s_scale;
         const int g_first = p_first + tok_of(g), g_last = g_first + kTok - 1;
+        const float below = fminf(kBelow + __log2f(static_cast<float>(max(tiles, 1))), kMostBelow);
         float m = kNegRef, top = kNegRef, l = 0.0f;  // reference, maximum, sum
         bool ok = true;
         if ((g == 0 || two) && nt > 0) {
@@ -442,12 +444,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int e = 3; e < 15; e += 2) mx[c] = max3(mx[c], v(e), v(e + 1));
                     mx[c] = fmaxf(mx[c], v(15));
                 }
-                // A new reference lies 2^kBelow below the row's maximum and serves until a score lies 2^kLazy above it.  So the
-                // row's largest p is 2^8 or more, and FP16's smallest step 2^-32 of it: thousands of keys may lie 2^-20 below
-                // one that draws the weight and still carry the output, when that one's value is small.  (References 2^4
-                // above the maximum lost such keys, 1.5 % of a row of 8192, and saved moves: 8192 tokens full 579 us against
-                // 607, three documents under a window 333 and 356.  Moving to the half tile's maximum instead of the row's:
-                // 635 and 359 us.)
+                // A new reference lies 2^below below the row's maximum and serves until a score lies 2^kLazy above it: the row's
+                // largest p is between the two, and FP16's rounding at its small end, 2^-25, times the number of keys is 2^-20 of
+                // the largest weight at any length (from 262144 keys on more).  That much, because thousands of keys may lie
+                // 2^-20 below one that draws the weight and still carry the output, when that one's value is small.  (References
+                // 2^4 above the maximum lost such keys, up to 9.7 % of a row of 8192, and saved moves: 8192 tokens full 585 us
+                // against 608, three documents under a window 333 and 347, 16 mixed prompts 286 and 298.  Moving to the half
+                // tile's maximum instead of the row's costs as much again.)
                 const float tops = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
                 top = fmaxf(top, tops);
                 // Rows behind the unit's last token (the next request's, or a padding row's leftovers) move nothing: the bits of
@@ -456,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (__any_sync(0xffffffffu, move)) {
                     // all of the warp's rows move up, not only those that must: four sinks first leave 32 low references, and
                     // one of the rows outgrew its own in most of the following steps
-                    const float m_new = fmaxf(m, top - kBelow);
+                    const float m_new = fmaxf(m, top - below);
                     const float alpha = ex2(m - m_new);
                     m = m_new;
                     l *= alpha;

@@ -7,8 +7,8 @@ scores are zero for every head.  Queries are 5.47 x (+-1), which BF16 rounds to 
 its step, so no rounding falls the other way than in 64 bits.
 
 Tolerances: those of tests/test_gpu_prompt.py without the allowance for queries (none differs): probabilities are off by 2^-12 of
-their value, independently, or by half of FP16's smallest step, 2^-25 against a largest of 2^8 or more, so 8232 keys by 9.6e-7 of
-the largest weight in all; a row is at least 0.002 of it (key 0's own value), so that is 5e-4 of the row.  The rest is the
+their value, independently, or by half of FP16's smallest step, which for all keys together is 2^-20 (9.5e-7) of the largest
+weight; a row is at least 0.002 of it (key 0's own value), so that is 5e-4 of the row.  The rest is the
 output's rounding to BF16, 2^-8 of an element at most and 1.6e-3 rms: a row is off by 3e-3 of its norm at most, an element by
 2^-7 of itself and 2e-3 (rows have elements of 0.7)."""
 import pytest
@@ -101,3 +101,17 @@ def test_steps_with_a_first_token_that_stays_visible(q_len, chunks, sinks, nats)
     abi.status_for("cuda").raise_if_set("attention")
     row, element = off(out, data)
     assert row < 5e-3 and element < 3.5e-3, (row, element)
+
+
+@pytest.mark.parametrize("ctx,new", [(100, 5), (600, 40), (2000, 20), (66000, 20), (66000, 40)])
+def test_prompt_keeps_them_at_any_length(ctx, new):
+    """The rounding of the smallest probabilities, times the keys there are, is 2^-20 of the largest weight."""
+    from muse_spark_open_b200 import abi, attention
+    for nats in (12.0, 15.0, 18.0):
+        data = far_weights([ctx], new, 7, nats=nats)
+        for splits in (0, 1):
+            out = attention.prompt_fn(oattn.to_device(data, "cuda"), splits=splits)
+            torch.cuda.synchronize()
+            abi.status_for("cuda").raise_if_set("attention")
+            row, element = off(out, data)
+            assert row < 3e-3 and element < 2e-3, (nats, splits, row, element)
