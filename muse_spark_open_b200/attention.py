@@ -8,8 +8,8 @@ q_len is 1 (decode) or 8 (verify) as in the reference, or any other length: bloc
 a window and sinks, write the new rows where the page table says (cache_loc says the same in the reference, submission.py:37-65).
 RoPE's angle is the reference's product in 32 bits for tokens and blocks of 8 without sinks, off by up to 2^-11 rad at positions
 8192 to 16384 and twice that at twice the position; prompts, other blocks and steps with sinks turn by the exact one.  They may
-share a cache: each key has its own token's angle either way, and the two differ by less than the queries' other roundings move
-a score.
+share a cache: each key has its own token's angle either way, and at position 16384 the two differ by about as much of a score
+as the queries' other roundings do.
 Nothing derived from `data` is cached between calls; only the RoPE frequency table (a function of
 theta and head_dim) is kept per device.
 """
@@ -78,7 +78,7 @@ def kernel_fn(data: dict, chunks: int = 0, stages: int = 0) -> torch.Tensor:
     out = torch.empty((b, l, wide), dtype=torch.bfloat16, device=qkv.device)
     if l != 1 and (l != 8 or (cfg["window"] and cfg.get("sinks", 0))) and not chunks and not stages:
         # blocks of other lengths, and verify blocks with sinks: the prompt kernels (16 requests x 8 tokens, window 1024 + 4
-        # sinks: 21 us against 51 us for the verify kernel, whose results without sinks stay what they were)
+        # sinks, in a graph: 22 us against 52 us for the verify kernel, whose results without sinks stay what they were)
         _run_prompt(data, cfg, qkv, b * l, cols, ld, out, wide, None, l, 0)
         return out
     _run_step(abi.ptr(qkv), ld, out.data_ptr(), wide, data, cfg, qkv.get_device(), chunks, stages, 0, False, 0)

@@ -25,14 +25,16 @@
 // waited 1300 clocks for its next scores, a third of the loop; a third row tile does not fit.)
 // Values are 0 * V for the tokens that do not see them, so a NaN among them is zeroed where not all tokens of the unit see it,
 // and the rows that do are made NaN at the end.
-// Measured (32 + 4 heads): 8192 tokens, full, behind nothing: 537 us = 1.02 PFLOP/s, 62 % of the rate of a BF16 matrix product;
-// three documents of 2500 to 4099 tokens under window 1024 + 64 sinks 330 us, 0.49 PFLOP/s of visible keys; 16 prompts of 1 to
-// 1024 tokens under window 1024 + 4 284 us; 16 x 8 tokens 21 us; 19 tokens behind 7001 cached ones 14.5 us.  Bound by the two
-// softmax warps of each scheduler: 1750 - 1850 clocks per 64 keys and two row tiles, of which a loop of the softmax alone
-// (scores from TMEM, maximum, exponentials, back to TMEM) takes 1500 on the scheduler that also issues the products; tensor
-// cores and special-function units are a third busy each.  Per unit come 12 us: 3 until the first scores, 2 for the last product,
-// 5.5 for norm, gate and stores, 1 until the next CTA runs.  Under a window a unit has only 5 to 40 tiles, so these and the
-// masked parts of its edge tiles weigh more.  Small calls: prep 3 us, main from 6, combine 1, and 1.5 us between the launches.
+// Measured (32 + 4 heads, replayed in a graph / called from Python): 8192 tokens, full, behind nothing: 564 / 610 us = 0.97 /
+// 0.90 PFLOP/s, 59 / 55 % of the rate of a BF16 matrix product; three documents of 2500 to 4099 tokens under window 1024 + 64
+// sinks 345 / 347 us, 0.47 PFLOP/s of visible keys; 16 prompts of 1 to 1024 tokens under window 1024 + 4 294 / 297 us; 16 x 8
+// tokens 22 / 25 us; 19 tokens behind 7001 cached ones 14.7 / 18.9 us.  No unit is near its limit (tensor cores and
+// special-function units a third busy each); the time goes with the chain of the two softmax warps of each scheduler: 1750 - 1850
+// clocks per 64 keys and two row tiles, of which a loop of the softmax alone (scores from TMEM, maximum, exponentials, back to
+// TMEM) takes 1500 on the scheduler that also issues the products.  Per unit come 12 us: 3 until the first scores, 2 for the
+// last product, 5.5 for norm, gate and stores, 1 until the next CTA runs.  Under a window a unit has only 5 to 40 tiles, so
+// these and the masked parts of its edge tiles weigh more.  Small calls: prep 3 us, main from 6, combine 1, and 1.5 us between the
+// launches.
 // Tried without gain: an MMA warp per row tile, a reference without a maximum, turn-taking softmax warps, scores fetched a
 // half ahead, a persistent grid, output tiles stored by TMA, four softmax warpgroups, more polynomials; for units with one
 // row tile, half of each tile's keys for each group of softmax warps (16 x 8 tokens: 22.6 us).

@@ -5,7 +5,8 @@ max_pages] (-1 = no page), seq_lens int32 [rows] (tokens in the cache), refs int
 page; 0 = free), and page_size.  A row is one request; `pool["page_table"]` and `pool["seq_lens"]` (or some of their rows)
 go into the `data` of attention.kernel_fn / prompt_fn and layer.kernel_fn as they are.  Lists of rows are int32 device
 tensors.  `caches` are the tensors whose first axis is the physical page and whose second the slot, K and V of every layer
-that uses the pool.  A step of a serving loop:
+that uses the pool: at most 128 per call (64 layers), all with the same bytes per token, a multiple of 16, because fork and
+compact change the table in the call that moves the data.  A step of a serving loop:
 
     loc = pages.extend(pool, rows, q_len)                 # room for the next tokens; their cache rows
     ... attention / layer step with pool["page_table"], pool["seq_lens"], cache_loc=loc ...
@@ -13,8 +14,7 @@ that uses the pool.  A step of a serving loop:
     pages.trim(pool, rows, window, sinks)                 # what the window has passed goes back
 
 Everything happens on the device, in place and in stream order (order the streams yourself when you use several on one pool);
-nothing is read back, so all calls can be captured in a CUDA
-graph.  New pages are the lowest free ones, given out in the order of the rows: results do not depend on scheduling.
+nothing is read back, so all calls can be captured in a CUDA graph.  New pages are the lowest free ones, given out in the order of the rows: results do not depend on scheduling.
 Problems with the contents (a row out of range or listed twice, no free page, seq_lens set back into pages that a fork shares
 and then extended, cu_seqlens that falls or names more tokens than `tokens`, negative seq_lens) are reported in the status
 word (`abi.status_for(device).raise_if_set()`), and the entries concerned are skipped; include/msk.h says how.

@@ -3,8 +3,8 @@ output is carried by thousands of keys whose weights lie 2^-14 to 2^-26 below th
 
 Every query head is a vector of equal magnitudes, s with its first m entries' signs flipped, so q . k0 for k0 along s falls
 linearly with m: eight heads see key 0 from 16 down to 8 nats above the others.  New keys alternate against s in pairs, their
-scores are zero for every head.  Queries are 5.47 x (+-1), which BF16 rounds to 5.46875 = 5.5 - 2^-5 with 2^-5 to either border of
-its step, so no rounding falls the other way than in 64 bits.
+scores are zero for every head.  Queries are 5.4730 x (+-1), 0.004 from BF16's 5.46875 and 0.011 from the border of its step, so
+no rounding falls the other way than in 64 bits.
 
 Tolerances: those of tests/test_gpu_prompt.py without the allowance for queries (none differs): probabilities are off by 2^-12 of
 their value, independently, or by half of FP16's smallest step, which for all keys together is 2^-20 (9.5e-7) of the largest
