@@ -14,7 +14,7 @@ def test_which_kernels_a_block_takes(monkeypatch, q_len, window, sinks, took):
     monkeypatch.setattr(attention, "_run_step", lambda *a: calls.append("step"))
     monkeypatch.setattr(attention, "_run_prompt", lambda *a: calls.append("prompt"))
     cfg = {"batch": 2, "q_len": q_len, "num_q_heads": 8, "head_dim": 128, "window": window, "sinks": sinks}
-    data = {"config": cfg, "qkv": torch.zeros(2, q_len, 18 * 128, dtype=torch.bfloat16), "k_cache": torch.zeros(1).to(torch.float8_e4m3fn),
+    data = {"config": cfg, "qkv": torch.empty(2, q_len, 18 * 128, dtype=torch.bfloat16), "k_cache": torch.zeros(1).to(torch.float8_e4m3fn),
             "seq_lens": torch.zeros(2, dtype=torch.int32), "page_table": torch.zeros(2, 1, dtype=torch.int32),
             "cache_loc": torch.zeros(2 * q_len, dtype=torch.int64)}
     monkeypatch.setattr(attention.abi, "ptr", lambda t: t.data_ptr())
